@@ -44,7 +44,10 @@ def _parse_structs(text: str) -> dict[str, type]:
     for body, name in re.findall(r"typedef\s+struct\s*\{(.*?)\}\s*(\w+)\s*;", text, flags=re.S):
         fields = []
         for decl in filter(None, (d.strip() for d in body.split(";"))):
-            m = re.match(r"((?:unsigned\s+long\s+long)|(?:unsigned\s+short)|\w+)\s+(.*)$", decl, flags=re.S)
+            if "*" in decl:  # a pointer field: one name, any pointee
+                fields.append((re.search(r"(\w+)\s*$", decl).group(1), ctypes.c_void_p))
+                continue
+            m = re.match(r"((?:(?:unsigned\s+)?long\s+long)|(?:unsigned\s+short)|\w+)\s+(.*)$", decl, flags=re.S)
             base = _SCALARS[" ".join(m.group(1).split())]
             for item in (i.strip() for i in m.group(2).split(",")):
                 arr = re.match(r"(\w+)\s*\[\s*(\d+)\s*\]", item)

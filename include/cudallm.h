@@ -243,6 +243,163 @@ int cudallm_kernel_gemm(const unsigned short* w, const unsigned short* x, const 
 int cudallm_attention_noalloc(const float* q, const unsigned short* k_cache, const unsigned short* v_cache, int ctx,
                               float* out, int nh, int nkv, int hd, int max_seq, void* stream);
 
+/* ---- paged key-value cache and beam search (no counterpart in the reference, whose engine keeps one contiguous
+ * cache and decodes greedily). Every pointer inside these argument structs is caller-owned DEVICE memory; the
+ * calls only enqueue work on `stream` (a cudaStream_t of the current device, NULL = the legacy default stream),
+ * allocate nothing and can be captured in a CUDA graph. Argument errors are INVALID_ARG and enqueue nothing.
+ * What the host cannot see (lengths, tables, positions, parents) is bounded inside the kernels as stated below,
+ * so no content of those arrays leads to an access outside of the caller's buffers.
+ *
+ * Workspaces: `workspace` points to at least cudallm_*_workspace_bytes() bytes, 256-byte aligned, whose first
+ * CUDALLM_WORKSPACE_COUNTERS bytes the caller sets to zero once, when it is allocated; every call leaves them zero. A workspace may serve
+ * all of these calls, one after the other on one stream; calls that may overlap (other streams) need their own. */
+
+#define CUDALLM_WORKSPACE_COUNTERS 16384
+
+#define CUDALLM_X_FP32 0
+#define CUDALLM_X_FP16 1
+#define CUDALLM_X_BF16 2
+
+/* A pool of pages: k and v are [n_layers][n_pages][n_kv_heads][page_size][head_dim] with the strides below (in
+ * elements, the same for both, multiples of 8; head_dim is contiguous), 16-byte aligned. head_dim: a multiple of 8,
+ * 8 .. 256. A table row lists the pages of one sequence's tokens 0 .. page_size-1, page_size .. and so on; an entry
+ * outside [0, n_pages) holds no page: attention treats its tokens as masked, append stores nothing there. */
+typedef struct {
+    int struct_size; /* sizeof(cudallm_pages) */
+    int kv_dtype;    /* CUDALLM_KV_FP16 or CUDALLM_KV_BF16 */
+    int n_layers, n_pages, n_kv_heads, page_size, head_dim, reserved;
+    void* k;
+    void* v;
+    long long layer_stride, page_stride, head_stride, token_stride;
+} cudallm_pages;
+
+/* Attention of one new token per sequence over its pages: out[b][h] = softmax_t(scale q.k_t) v over the cached
+ * positions max(0, lens[b] - window) <= t < lens[b] (window 0: all; lens outside [0, table_width * page_size] are
+ * clamped to it) whose page exists; n_heads / n_kv_heads query heads share a key head. lse (or NULL): the natural
+ * logarithm of the sum of the exponentials. No position left: out 0, lse -inf. Scores, statistics and sums are fp32.
+ * q [n_seq][n_heads][head_dim] has its own strides, out and lse are contiguous; out has q's type and must not
+ * overlap q. Values in unused slots of a page do not matter; keys and values of used ones must be finite. */
+typedef struct {
+    int struct_size; /* sizeof(cudallm_attend_args) */
+    int layer, x_dtype, n_seq, n_heads, table_width, window;
+    float scale;
+    const void* q;
+    long long q_seq_stride, q_head_stride; /* elements */
+    const int* tables;                     /* [n_seq][table_width] */
+    long long table_stride;                /* elements */
+    const int* lens;                       /* [n_seq] */
+    void* out;                             /* [n_seq][n_heads][head_dim] */
+    float* lse;                            /* [n_seq][n_heads] or NULL */
+    void* workspace;
+    unsigned long long workspace_bytes;
+} cudallm_attend_args;
+
+int cudallm_paged_attend(const cudallm_pages* pages, const cudallm_attend_args* args, void* stream);
+/* Workspace of cudallm_paged_attend for any arguments (a constant). */
+unsigned long long cudallm_attend_workspace_bytes(void);
+
+/* Rotary positions of n_tokens new tokens: q_out = rotated q (may be q itself); rotated k and v are stored in the
+ * slots of their positions. Token i belongs to table row rows[i] (rows NULL: row i) at positions[i]. Pair j < rotary
+ * / 2 of a head turns by the angle (float)position * inv_freq[j], rounded to fp32 as in the decode step, with cos and
+ * sin multiplied by `factor`; the pair is dims (j, j + rotary / 2), or (2j, 2j + 1) with interleaved != 0; dims from
+ * `rotary` on are copied. A negative position is padding: q_out is 0 there and nothing is stored; nothing is stored
+ * either for a row outside [0, n_rows), a position beyond the table or an entry without a page. Two tokens of one call
+ * must not share a slot. rotary 0 stores without rotation. q may be NULL (keys and values only). */
+typedef struct {
+    int struct_size; /* sizeof(cudallm_append_args) */
+    int layer, x_dtype, n_tokens, n_heads, n_rows, table_width, rotary, interleaved;
+    float factor;
+    const void* q;
+    const void* k;
+    const void* v;
+    long long q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    const float* inv_freq; /* [rotary / 2] */
+    const int* positions;  /* [n_tokens] */
+    const int* rows;       /* [n_tokens] or NULL */
+    const int* tables;     /* [n_rows][table_width] */
+    long long table_stride;
+    void* q_out;           /* [n_tokens][n_heads][head_dim], strides below */
+    long long out_token_stride, out_head_stride;
+} cudallm_append_args;
+
+int cudallm_paged_append(const cudallm_pages* pages, const cudallm_append_args* args, void* stream);
+
+/* The next step's sequences: row i of tables_out continues row parents[i] of tables (a parent outside [0, n_rows):
+ * row i is empty, which is how sequences are freed). Full pages are shared. The first child (lowest i) of a
+ * parent also takes over the parent's pages from the first not full one on, if no other row refers to that one; any
+ * other child gets a page of its own with a copy of the tokens in that page, in every layer. Then every row gets the
+ * pages that `room` more tokens need. New pages are the lowest-numbered ones with refs 0, handed out in row order;
+ * refs_out counts each page's references after the call (references that are not in `tables` stay counted).
+ * A row's entries end at the first one without a page at or after its full pages. lens are clamped to
+ * [0, table_width * page_size]. *missing = how many pages were wanted and not found (0 = success); their entries are
+ * -1. The inputs stay as they are (outputs must not overlap them), so after a shortage the caller frees rows and calls
+ * again on the same inputs. Layers' pages with refs > 0 are not written. */
+typedef struct {
+    int struct_size; /* sizeof(cudallm_fork_args) */
+    int n_rows, n_out, table_width, room, reserved;
+    const int* tables; /* [n_rows][table_width] */
+    long long table_stride;
+    const int* lens;    /* [n_rows] */
+    const int* refs;    /* [n_pages] */
+    const int* parents; /* [n_out] */
+    int* tables_out;    /* [n_out][table_width] */
+    long long table_out_stride;
+    int* lens_out; /* [n_out] */
+    int* refs_out; /* [n_pages] */
+    int* missing;  /* [1] */
+    void* workspace;
+    unsigned long long workspace_bytes;
+} cudallm_fork_args;
+
+int cudallm_paged_fork(const cudallm_pages* pages, const cudallm_fork_args* args, void* stream);
+
+/* Moves the *live pages with refs > 0 to the front of the pool: the k-th lowest unused page among the first *live takes
+ * content (all layers), references and table entries of the k-th lowest used page after them. Table entries without a
+ * page become -1. tables and refs stay as they are (outputs must not overlap them); pages from *live on may be
+ * given back or reused afterwards. */
+typedef struct {
+    int struct_size; /* sizeof(cudallm_compact_args) */
+    int n_rows, table_width, reserved;
+    const int* tables;
+    long long table_stride;
+    const int* refs; /* [n_pages] */
+    int* tables_out;
+    long long table_out_stride;
+    int* refs_out; /* [n_pages] */
+    int* live;     /* [1] */
+    void* workspace;
+    unsigned long long workspace_bytes;
+} cudallm_compact_args;
+
+int cudallm_paged_compact(const cudallm_pages* pages, const cudallm_compact_args* args, void* stream);
+/* Workspace of cudallm_paged_fork and cudallm_paged_compact for pools of n_pages pages and calls of up to `rows`
+ * rows (the larger of n_rows and n_out); 0 for sizes that the calls refuse. */
+unsigned long long cudallm_pages_workspace_bytes(int n_pages, int rows);
+
+/* Beam search's selection. Candidate (w, t) of group g: scores[g][w] + (x[t] - logsumexp(x)) with x = row g * beams +
+ * w of logits, or, where finished[g][w] != 0 (finished may be NULL), x = 0 at eos and -inf elsewhere. A candidate that
+ * is not a number counts as -inf. The `keep` best of each group, in order: larger candidate, then lower beam, then
+ * larger logit (one that is not a number: -inf), then lower token. out_parents are rows of logits (as
+ * cudallm_paged_fork takes them). beams 1 .. 64, keep 1 .. 64 and at most beams * vocab. */
+typedef struct {
+    int struct_size; /* sizeof(cudallm_beam_args) */
+    int x_dtype, n_groups, beams, keep, vocab, eos, reserved;
+    const void* logits; /* [n_groups * beams][vocab] */
+    long long row_stride;
+    const float* scores;  /* [n_groups][beams] */
+    const int* finished;  /* [n_groups][beams] or NULL */
+    float* out_scores;    /* [n_groups][keep] */
+    int* out_parents;     /* [n_groups][keep] */
+    int* out_tokens;      /* [n_groups][keep] */
+    void* workspace;
+    unsigned long long workspace_bytes;
+} cudallm_beam_args;
+
+int cudallm_beam_select(const cudallm_beam_args* args, void* stream);
+/* Workspace of cudallm_beam_select for up to `rows` = n_groups * beams rows of up to vocab logits; 0 for sizes that
+ * the call refuses. */
+unsigned long long cudallm_beam_workspace_bytes(int rows, int vocab, int keep);
+
 #ifdef __cplusplus
 }
 #endif

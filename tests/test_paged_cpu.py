@@ -1,0 +1,159 @@
+"""CPU: host-side argument checks of the paged cache and of beam search's selection through the C ABI (they come
+before any CUDA call), and the oracle's own invariants."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from cudallm_b200 import abi, paged
+from oracle import paged64 as R
+
+FAKE = 1 << 20  # an aligned address that nothing reads: every call here is refused
+
+
+@pytest.fixture(autouse=True)
+def _lib(native_lib):
+    return native_lib
+
+
+def _struct(name, **fields):
+    a = abi.struct(name)()
+    a.struct_size = ctypes.sizeof(a)
+    for k, v in fields.items():
+        setattr(a, k, v)
+    return a
+
+
+def _pages(**over):
+    f = dict(kv_dtype=0, n_layers=2, n_pages=8, n_kv_heads=2, page_size=16, head_dim=64, k=FAKE, v=FAKE, layer_stride=16384, page_stride=2048,
+             head_stride=1024, token_stride=64)
+    return _struct("cudallm_pages", **{**f, **over})
+
+
+def _attend(**over):
+    f = dict(layer=0, x_dtype=0, n_seq=2, n_heads=4, table_width=3, window=0, scale=0.125, q=FAKE, q_seq_stride=256, q_head_stride=64, tables=FAKE,
+             table_stride=3, lens=FAKE, out=2 * FAKE, workspace=FAKE, workspace_bytes=1 << 40)
+    return _struct("cudallm_attend_args", **{**f, **over})
+
+
+def _append(**over):
+    f = dict(layer=0, x_dtype=0, n_tokens=2, n_heads=4, n_rows=2, table_width=3, rotary=64, interleaved=0, factor=1.0, q=FAKE, k=FAKE, v=FAKE,
+             q_token_stride=256, q_head_stride=64, inv_freq=FAKE, positions=FAKE, tables=FAKE, table_stride=3, q_out=FAKE, out_token_stride=256,
+             out_head_stride=64)
+    return _struct("cudallm_append_args", **{**f, **over})
+
+
+def _fork(**over):
+    f = dict(n_rows=2, n_out=2, table_width=3, room=1, tables=FAKE, table_stride=3, lens=2 * FAKE, refs=3 * FAKE, parents=4 * FAKE, tables_out=5 * FAKE,
+             table_out_stride=3, lens_out=6 * FAKE, refs_out=7 * FAKE, missing=8 * FAKE, workspace=9 * FAKE, workspace_bytes=1 << 40)
+    return _struct("cudallm_fork_args", **{**f, **over})
+
+
+def _compact(**over):
+    f = dict(n_rows=2, table_width=3, tables=FAKE, table_stride=3, refs=3 * FAKE, tables_out=5 * FAKE, table_out_stride=3, refs_out=7 * FAKE,
+             live=8 * FAKE, workspace=9 * FAKE, workspace_bytes=1 << 40)
+    return _struct("cudallm_compact_args", **{**f, **over})
+
+
+def _beam(**over):
+    f = dict(x_dtype=0, n_groups=2, beams=4, keep=4, vocab=100, eos=0, logits=FAKE, row_stride=100, scores=FAKE, out_scores=FAKE, out_parents=FAKE,
+             out_tokens=FAKE, workspace=FAKE, workspace_bytes=1 << 40)
+    return _struct("cudallm_beam_args", **{**f, **over})
+
+
+def _refused(lib, fn, *structs) -> bool:
+    return getattr(lib, fn)(*(None if s is None else ctypes.byref(s) for s in structs), None) == 1
+
+
+@pytest.mark.parametrize("over", [dict(struct_size=8), dict(kv_dtype=2), dict(n_pages=0), dict(page_size=-1), dict(head_dim=60), dict(head_dim=264), dict(k=None),
+                                  dict(v=FAKE + 8), dict(page_stride=1024), dict(token_stride=60), dict(token_stride=68), dict(layer_stride=-16384), dict(head_stride=0)],
+                         ids=str)
+def test_pools_that_are_refused(native_lib, over):
+    for fn, args in (("cudallm_paged_attend", _attend()), ("cudallm_paged_append", _append()), ("cudallm_paged_fork", _fork()),
+                     ("cudallm_paged_compact", _compact())):
+        assert _refused(native_lib, fn, _pages(**over), args), fn
+        assert _refused(native_lib, fn, None, args) and _refused(native_lib, fn, _pages(), None)
+
+
+@pytest.mark.parametrize("over", [dict(struct_size=0), dict(layer=2), dict(layer=-1), dict(x_dtype=3), dict(n_seq=-1), dict(n_seq=65537), dict(n_heads=0), dict(n_heads=5),
+                                  dict(window=-1), dict(scale=float("inf")), dict(q=None), dict(q=FAKE + 2), dict(lens=None), dict(out=None), dict(tables=None),
+                                  dict(table_stride=2), dict(table_width=-1), dict(table_width=1 << 28, table_stride=1 << 28), dict(out=FAKE + 1024), dict(q_seq_stride=-1),
+                                  dict(workspace=None), dict(workspace_bytes=100), dict(workspace=FAKE + 16), dict(lse=FAKE + 2)], ids=str)
+def test_attend_refusals(native_lib, over):
+    assert _refused(native_lib, "cudallm_paged_attend", _pages(), _attend(**over))
+
+
+@pytest.mark.parametrize("over", [dict(struct_size=0), dict(layer=9), dict(x_dtype=-1), dict(n_tokens=-1), dict(n_heads=0), dict(rotary=3), dict(rotary=66), dict(rotary=-2),
+                                  dict(inv_freq=None), dict(k=None), dict(v=None), dict(positions=None), dict(q_out=None), dict(factor=float("nan")),
+                                  dict(q_out=FAKE + 4), dict(out_head_stride=32), dict(out_token_stride=0), dict(k_head_stride=-8), dict(tables=None),
+                                  dict(out_token_stride=192), dict(rows=FAKE + 1)], ids=str)
+def test_append_refusals(native_lib, over):
+    assert _refused(native_lib, "cudallm_paged_append", _pages(), _append(**over))
+
+
+@pytest.mark.parametrize("over", [dict(struct_size=0), dict(n_rows=-1), dict(n_out=65537), dict(room=-1), dict(tables=None), dict(lens=None), dict(refs=None),
+                                  dict(parents=None), dict(tables_out=FAKE), dict(tables_out=FAKE + 20), dict(refs_out=3 * FAKE), dict(missing=3 * FAKE + 28),
+                                  dict(lens_out=5 * FAKE + 4), dict(missing=None), dict(workspace_bytes=0), dict(table_out_stride=1)], ids=str)
+def test_fork_refusals(native_lib, over):
+    assert _refused(native_lib, "cudallm_paged_fork", _pages(), _fork(**over))
+
+
+@pytest.mark.parametrize("over", [dict(struct_size=0), dict(n_rows=-1), dict(tables=None), dict(refs=None), dict(refs_out=3 * FAKE), dict(live=None), dict(live=7 * FAKE),
+                                  dict(tables_out=FAKE + 8), dict(workspace=None), dict(table_stride=0)], ids=str)
+def test_compact_refusals(native_lib, over):
+    assert _refused(native_lib, "cudallm_paged_compact", _pages(), _compact(**over))
+
+
+@pytest.mark.parametrize("over", [dict(struct_size=0), dict(x_dtype=3), dict(n_groups=-1), dict(n_groups=1 << 20), dict(beams=0), dict(beams=65), dict(keep=0), dict(keep=65),
+                                  dict(vocab=0), dict(beams=1, vocab=3, row_stride=3), dict(logits=None), dict(logits=FAKE + 2), dict(scores=None), dict(out_tokens=None),
+                                  dict(row_stride=99), dict(finished=FAKE, eos=100), dict(finished=FAKE, eos=-1), dict(workspace_bytes=8)], ids=str)
+def test_beam_refusals(native_lib, over):
+    assert _refused(native_lib, "cudallm_beam_select", _beam(**over))
+
+
+def test_messages_and_workspace_sizes(native_lib):
+    assert _refused(native_lib, "cudallm_paged_attend", _pages(), _attend(layer=7))
+    assert b"layer" in native_lib.cudallm_last_error()
+    counters = 16384
+    assert native_lib.cudallm_attend_workspace_bytes() >= counters
+    assert native_lib.cudallm_pages_workspace_bytes(1000, 64) > counters
+    assert native_lib.cudallm_pages_workspace_bytes(0, 64) == 0 and native_lib.cudallm_pages_workspace_bytes(8, 1 << 20) == 0
+    assert native_lib.cudallm_beam_workspace_bytes(64, 128256, 16) > counters and native_lib.cudallm_beam_workspace_bytes(4, 100, 65) == 0
+
+
+def test_tensors_off_the_gpu_are_refused():
+    k = torch.zeros((1, 2, 1, 8, 64), dtype=torch.float16)
+    with pytest.raises(paged.CudaLLMError):
+        paged.PagedCache(k, k)
+    with pytest.raises(paged.CudaLLMError):
+        paged.Rope(torch.zeros(4))
+    with pytest.raises(paged.CudaLLMError):
+        paged.Rope.make(63)
+    with pytest.raises(paged.CudaLLMError):
+        paged.beam_select(torch.zeros((2, 5)), torch.zeros((1, 2)), keep=1)
+
+
+def test_oracle_fork_keeps_references_and_contents():
+    """Walks of forks on random parents: references equal the tables' entries, and every row's tokens are its ancestor's."""
+    rng = np.random.default_rng(0)
+    page, pages = 4, 60
+    content = np.full((pages, page), -1)
+    tables, lens, refs = np.full((1, 12), -1), np.array([0]), np.zeros(pages, np.int64)
+    texts = [[]]
+    for step in range(25):
+        parents = rng.integers(0, len(lens), 4)
+        tables, lens, refs, missing, copies = R.fork_ref(tables, lens, refs, parents, page, 1)
+        assert missing == 0
+        for src, dst, n in copies:
+            content[dst, :n] = content[src, :n]
+        texts = [list(texts[p]) for p in parents]
+        for r in range(4):
+            content[tables[r][lens[r] // page], lens[r] % page] = 100 * step + r
+            texts[r].append(100 * step + r)
+            lens[r] += 1
+        assert np.array_equal(np.bincount(tables[tables >= 0], minlength=pages), refs)
+        for r in range(4):
+            assert [content[tables[r][t // page], t % page] for t in range(lens[r])] == texts[r]

@@ -1,0 +1,626 @@
+"""GPU: the paged cache's operators and beam search's selection (cudallm_b200/paged.py) against oracle/paged64.py.
+
+Tolerances (eps = 2^-24, one rounding to fp32; errors of a sum of n terms taken as sqrt(n) eps times its size, with a
+factor of 8 in hand):
+  attention   a score is off by E = 8 eps sqrt(D) S, S = scale sum |q k|; so is ln of every weight, twice over with the sum:
+              |out - ref| <= (2 E + 8 eps sqrt(T)) max|v|, |lse - ref| <= E + 8 eps sqrt(T) + 2 eps |lse|
+  rotation    |y - ref| <= 8 eps factor (|a| + |b|)
+  selection   |score - ref| <= 8 eps (|score| + |logit| + |lse| + sqrt(V))
+each plus half a unit in the last place of the output's type (2^-11 fp16, 2^-8 bf16 relative, 2^-24 absolute), and integers
+exactly."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from cudallm_b200 import paged
+from cudallm_b200.abi import CudaLLMError
+from oracle import paged64 as R
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+HALF_ULP = {torch.float32: EPS, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(autouse=True)
+def _lib(native_lib):
+    return native_lib
+
+
+def _np(t: torch.Tensor) -> np.ndarray:
+    return t.detach().cpu().double().numpy() if t.is_floating_point() else t.detach().cpu().numpy()
+
+
+def _ints(a) -> torch.Tensor:
+    return torch.from_numpy(np.array(a, np.int32)).cuda()
+
+
+def _within(x: torch.Tensor, ref: np.ndarray, tol: np.ndarray) -> None:
+    got = _np(x)
+    assert got.shape == ref.shape
+    assert np.array_equal(np.isfinite(got), np.isfinite(ref)) and np.array_equal(got[~np.isfinite(ref)], ref[~np.isfinite(ref)])
+    with np.errstate(invalid="ignore"):
+        off = np.abs(got - ref) - (tol + HALF_ULP[x.dtype] * np.abs(ref) + EPS)
+    off = np.where(np.isfinite(ref), off, 0.0)
+    assert off.max(initial=0.0) <= 0, f"over the tolerance by {off.max()}"
+
+
+def _cache(layers, pages, kv_heads, page, dim, dtype, order="heads", fill=None, seed=0):
+    shape = (layers, pages, kv_heads, page, dim) if order == "heads" else (layers, pages, page, kv_heads, dim)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    k, v = (torch.randn(shape, generator=gen, device="cuda").to(dtype) if fill is None else torch.full(shape, fill, dtype=dtype, device="cuda")
+            for _ in range(2))
+    if order != "heads":
+        k, v = k.transpose(2, 3), v.transpose(2, 3)
+    return paged.PagedCache(k, v)
+
+
+def _layout(lens, page, width=None, spare=2, seed=0):
+    """A table with pages of its own for every row, anywhere in the pool."""
+    counts = [-(-n // page) for n in lens]
+    width = max(counts + [1]) if width is None else width
+    pages = sum(counts) + spare
+    ids, t, at = np.random.default_rng(seed).permutation(pages), np.full((len(lens), width), -1, np.int32), 0
+    for r, n in enumerate(counts):
+        t[r, :n] = ids[at:at + n]
+        at += n
+    return t, pages
+
+
+def _poison(cache, table, lens, layer):
+    """Fills every slot that no row uses with NaN and infinities, so that a read of one shows."""
+    used = np.zeros((cache.n_pages, cache.page_size), bool)
+    for r, n in enumerate(lens):
+        for t in range(n):
+            if 0 <= table[r][t // cache.page_size] < cache.n_pages:
+                used[table[r][t // cache.page_size], t % cache.page_size] = True
+    dirt = torch.from_numpy(~used).cuda()[None, :, None, :, None]
+    cache.k.copy_(torch.where(dirt, float("nan"), cache.k))
+    cache.v.copy_(torch.where(dirt, float("inf"), cache.v))
+
+
+def _check_attend(cache, q, table, lens, *, layer=0, scale=None, window=0):
+    out, lse = cache.attend(q, _ints(table), _ints(lens), layer=layer, scale=scale, window=window, with_lse=True)
+    k = np.nan_to_num(_np(cache.k[layer]), nan=1e30, posinf=1e30)
+    v = np.nan_to_num(_np(cache.v[layer]), nan=1e30, posinf=1e30)
+    ref, ref_lse, size = R.attend64(_np(q), k, v, np.array(table), lens, scale, window)
+    T = max(1, cache.page_size * np.array(table).shape[1])
+    vmax = np.abs(np.where(v < 1e30, v, 0)).max()
+    e = 8 * EPS * np.sqrt(cache.head_dim) * size
+    _within(out, ref, ((2 * e + 8 * EPS * np.sqrt(T)) * vmax)[..., None])
+    _within(lse, ref_lse, e + 8 * EPS * np.sqrt(T) + 2 * EPS * np.abs(np.where(np.isfinite(ref_lse), ref_lse, 0)))
+    return out, lse
+
+
+# ---- attention --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("x, kv", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16), (F16, BF16), (BF16, F16)])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 64), (32, 4, 128), (8, 8, 64), (7, 1, 80), (16, 1, 64), (40, 1, 32), (6, 2, 256), (24, 2, 128), (3, 3, 8)])
+@pytest.mark.parametrize("order, page", [("heads", 16), ("tokens", 24)])
+def test_attend_types_and_heads(x, kv, heads, kv_heads, dim, order, page):
+    lens = [0, 1, page - 1, page, page + 1, 130, 515]
+    table, pages = _layout(lens, page)
+    cache = _cache(2, pages, kv_heads, page, dim, kv, order, seed=heads)
+    _poison(cache, table, lens, 1)
+    q = torch.randn((len(lens), heads, dim), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(x)
+    _check_attend(cache, q, table, lens, layer=1)
+
+
+@pytest.mark.parametrize("page", [1, 3, 8, 16, 31, 32, 33, 64, 128, 1000])
+@pytest.mark.parametrize("window", [0, 1, 17, 64, 100000])
+def test_attend_page_sizes_and_windows(page, window):
+    lens = [1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 300, 0, 1999]
+    table, pages = _layout(lens, page)
+    cache = _cache(1, pages, 2, page, 64, F16)
+    _poison(cache, table, lens, 0)
+    q = torch.randn((len(lens), 8, 64), device="cuda")
+    _check_attend(cache, q, table, lens, window=window)
+
+
+@pytest.mark.parametrize("lens", [[32768], [9000, 1, 20000, 0], [5] * 300, [700 + 3 * i for i in range(64)], [0, 0, 0]], ids=str)
+def test_attend_lengths(lens):
+    table, pages = _layout(lens, 64)
+    cache = _cache(1, pages, 2, 64, 64, BF16)
+    q = torch.randn((len(lens), 8, 64), device="cuda", dtype=BF16)
+    a = _check_attend(cache, q, table, lens)
+    b = cache.attend(q, _ints(table), _ints(lens), with_lse=True)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])  # the same bits every time
+
+
+def test_attend_missing_pages_are_masked():
+    lens, page = [200, 200, 64, 500, 77], 16
+    table, pages = _layout(lens, page)
+    table[0, 3] = -1
+    table[0, 0] = -7
+    table[1, :] = -1  # nothing left
+    table[2, :2] = [pages, 2 ** 31 - 1]
+    table[3, 5:30] = -2 ** 31
+    cache = _cache(1, pages, 2, page, 64, F16)
+    _check_attend(cache, torch.randn((5, 8, 64), device="cuda"), table, lens)
+
+
+def test_attend_clamps_lengths_to_the_table():
+    table, pages = _layout([40, 40, 40], 8, width=5)
+    cache = _cache(1, pages, 1, 8, 64, F16)
+    q = torch.randn((3, 4, 64), device="cuda")
+    _check_attend(cache, q, table, [10 ** 9, -5, -2 ** 31])
+
+
+def test_attend_empty_table_and_no_rows():
+    cache = _cache(1, 4, 1, 8, 64, F16)
+    out, lse = cache.attend(torch.ones((2, 4, 64), device="cuda"), _ints(np.zeros((2, 0))), _ints([0, 3]), with_lse=True)
+    assert torch.all(out == 0) and torch.all(torch.isneginf(lse))
+    assert cache.attend(torch.ones((0, 4, 64), device="cuda"), _ints(np.zeros((0, 3))), _ints([])).shape == (0, 4, 64)
+
+
+def test_attend_strided_and_broadcast_queries():
+    lens = [70, 5, 33]
+    table, pages = _layout(lens, 16)
+    cache = _cache(1, pages, 2, 16, 64, F16)
+    packed = torch.randn((3, 12, 64), device="cuda")
+    _check_attend(cache, packed[:, 2:10], table, lens)
+    _check_attend(cache, packed.view(-1)[5:5 + 3 * 700].view(3, 700)[:, 1:513].view(3, 8, 64), table, lens)  # rows of an odd stride, off alignment
+    _check_attend(cache, packed[:1, :1].expand(3, 8, 64), table, lens)
+    wide = torch.full((3, 9), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = _ints(table)
+    a = cache.attend(packed[:, :8], wide[:, :table.shape[1]], _ints(lens))
+    assert torch.equal(a, cache.attend(packed[:, :8].contiguous(), _ints(table), _ints(lens)))
+
+
+def test_attend_peaked_and_tiny_scores():
+    """One key far above the rest, at either end and inside; and scores of one size where the weights are all alike."""
+    lens = [900] * 4
+    table, pages = _layout(lens, 16)
+    cache = _cache(1, pages, 1, 16, 64, F16)
+    k = cache.k[0, :, 0]
+    for r, t in enumerate([0, 450, 899]):
+        k[int(table[r][t // 16]), t % 16] = 6.0
+    for p in table[3]:
+        k[int(p)] = 0.0
+    q = torch.full((4, 8, 64), 3.0, device="cuda")
+    _check_attend(cache, q, table, lens)
+    _check_attend(cache, 200 * q, table, lens)
+    _check_attend(cache, q, table, lens, scale=0.0)
+    _check_attend(cache, q, table, lens, scale=-0.05)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 3e4, 1e6])
+def test_attend_query_magnitudes(size):
+    """fp32 queries far outside of the cache type's range; the scale brings the scores back."""
+    lens = [333, 50]
+    table, pages = _layout(lens, 16)
+    cache = _cache(1, pages, 2, 16, 64, F16)
+    q = size * torch.randn((2, 8, 64), device="cuda")
+    q[:, ::2] *= 1e-3
+    _check_attend(cache, q, table, lens, scale=0.125 / size)
+
+
+def test_attend_offsets_past_32_bits():
+    """Pages more than 2^32 elements into the pool."""
+    page, dim, pages = 64, 128, 2 ** 32 // (64 * 128) + 300
+    k = torch.empty((1, pages, 1, page, dim), dtype=F16, device="cuda")
+    ids = [pages - 1, 3, pages - 200, 2 ** 31 // (64 * 128) + 1]
+    k[0, ids] = torch.randn((4, 1, page, dim), device="cuda", dtype=F16)
+    cache = paged.PagedCache(k, k)
+    q = torch.randn((1, 4, dim), device="cuda")
+    out = cache.attend(q, _ints([ids]), _ints([250]))
+    small = k[:, ids].contiguous()
+    ref = paged.PagedCache(small, small).attend(q, _ints([[0, 1, 2, 3]]), _ints([250]))
+    assert torch.equal(out, ref)
+
+
+def test_attend_on_a_stream_of_its_own_and_in_a_graph():
+    lens = [3000, 10, 777]
+    table, pages = _layout(lens, 16)
+    cache = _cache(1, pages, 2, 16, 64, F16)
+    q, t, n = torch.randn((3, 8, 64), device="cuda"), _ints(table), _ints(lens)
+    ref = cache.attend(q, t, n)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        outs = [cache.attend(q, t, n) for _ in range(20)]
+    here = [cache.attend(q, t, n) for _ in range(20)]  # both streams at once
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref) for o in outs + here)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attend(q, t, n)
+        out2 = cache.attend(q, t, n, window=100)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref) and torch.equal(out2, cache.attend(q, t, n, window=100))
+
+
+# ---- rotary positions and the store to pages ----------------------------------------------------
+
+def _check_append(cache, q, k, v, positions, table, rope, *, layer=0, rows=None, out=None):
+    before_k, before_v = _np(cache.k).copy(), _np(cache.v).copy()
+    q0, k0, v0 = (None if x is None else _np(x).copy() for x in (q, k, v))
+    got = cache.append(q, k, v, _ints(positions), _ints(table), rope, layer=layer, rows=None if rows is None else _ints(rows), out=out)
+    pos = np.array(positions, np.int64)
+    inv = _np(rope.inv_freq) if rope else np.zeros(0)
+    factor = rope.factor if rope else 1.0
+    turn = lambda x: R.rotate64(x, pos, inv, rope is not None and rope.interleaved, factor)  # noqa: E731
+
+    def tol(x):
+        n = len(inv)
+        t = np.zeros_like(x)
+        i, j = (slice(0, 2 * n, 2), slice(1, 2 * n, 2)) if rope is not None and rope.interleaved else (slice(0, n), slice(n, 2 * n))
+        t[..., i] = t[..., j] = 8 * EPS * abs(factor) * (np.abs(x[..., i]) + np.abs(x[..., j]))
+        return t
+
+    if q is not None:
+        _within(got, np.where((pos >= 0)[:, None, None], turn(q0), 0.0), tol(q0))
+    k_tol, v_tol = np.zeros_like(before_k), np.zeros_like(before_v)
+    rk, tk = turn(k0), tol(k0)
+    for i, p in enumerate(pos):
+        row = i if rows is None else rows[i]
+        if p < 0 or not 0 <= row < len(table) or p // cache.page_size >= table.shape[1]:
+            continue
+        e = table[row][p // cache.page_size]
+        if 0 <= e < cache.n_pages:
+            before_k[layer, e, :, p % cache.page_size], k_tol[layer, e, :, p % cache.page_size] = rk[i], tk[i]
+            before_v[layer, e, :, p % cache.page_size] = v0[i]
+    if rope is None:
+        before_k = _np(torch.from_numpy(before_k).to(cache.k.dtype))
+    _within(cache.k, before_k, k_tol)
+    np.testing.assert_array_equal(_np(cache.v), _np(torch.from_numpy(before_v).to(cache.v.dtype)))
+
+
+@pytest.mark.parametrize("x, kv", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16), (BF16, F16)])
+@pytest.mark.parametrize("dim, rotary", [(64, 64), (128, 64), (80, 40), (64, 2), (256, 256), (8, 8), (48, 0)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("order", ["heads", "tokens"])
+def test_append_layouts(x, kv, dim, rotary, interleaved, order):
+    lens = [40, 33]
+    table, pages = _layout([n + 5 for n in lens], 16)
+    cache = _cache(2, pages, 2, 16, dim, kv, order)
+    pos = [p for n in lens for p in range(n)]
+    rows = [r for r, n in enumerate(lens) for _ in range(n)]
+    qkv = torch.randn((len(pos), 7 + 2 + 2, dim), device="cuda").to(x)
+    rope = paged.Rope.make(rotary, interleaved=interleaved, scaling="yarn", scale=8.0) if rotary else None
+    _check_append(cache, qkv[:, :7], qkv[:, 7:9], qkv[:, 9:], pos, table, rope, layer=1, rows=rows)
+
+
+@pytest.mark.parametrize("dim, offset, stride", [(64, 0, 64), (64, 1, 65), (64, 4, 68), (72, 2, 74), (64, 8, 72)])
+def test_append_strides_and_in_place(dim, offset, stride):
+    """Inputs off 16-byte alignment and with gaps between heads; q rotated in place and into a strided output."""
+    n, heads = 19, 5
+    table, pages = _layout([n], 8)
+    cache = _cache(1, pages, 1, 8, dim, F16)
+
+    def strided(h):
+        return torch.randn(offset + n * h * stride, device="cuda", dtype=F16)[offset:].view(n, h, stride)[..., :dim]
+
+    rope = paged.Rope.make(dim // 2 * 2)
+    q, k, v = strided(heads), strided(1), strided(1)
+    rows = [0] * n
+    out = strided(heads)
+    _check_append(cache, q, k, v, list(range(n)), table, rope, rows=rows, out=out)
+    _check_append(cache, q, k, v, list(range(n)), table, rope, rows=rows, out=q)
+    _check_append(cache, None, k, v, list(range(n)), table, rope, rows=rows)
+
+
+def test_append_one_token_a_row_padding_and_places_outside():
+    table, pages = _layout([64] * 6, 16)
+    table[2, 1] = -1
+    table[3, 0] = pages
+    cache = _cache(1, pages, 2, 16, 64, BF16)
+    q, k, v = (torch.randn((6, h, 64), device="cuda") for h in (8, 2, 2))
+    rope = paged.Rope.make(64)
+    _check_append(cache, q, k, v, [0, -1, 17, 3, 64, 2 ** 31 - 1], table, rope)
+    _check_append(cache, q, k, v, [5, -2 ** 31, 7, 8, 9, 10], table, rope, rows=[0, 1, -1, 6, 2 ** 31 - 1, 5])
+
+
+@pytest.mark.parametrize("scaling", ["none", "linear", "llama3", "yarn"])
+def test_append_long_positions(scaling):
+    """Angles of a million radians, where the reduction to one turn decides; the angle itself is rounded to fp32 by definition."""
+    pos = [0, 1, 104857, 105615, 105616, 131071, 999983, 2 ** 24 - 1]
+    cache = _cache(1, 2, 1, 8, 64, F16)
+    table = np.full((1, 2 ** 21), -1, np.int32)
+    q, k, v = (torch.randn((8, h, 64), device="cuda") for h in (4, 1, 1))
+    _check_append(cache, q, k, v, pos, table, paged.Rope.make(64, scaling=scaling, scale=32.0), rows=[0] * 8)
+
+
+def test_append_many_tokens_and_none():
+    lens = [1500, 1, 700]
+    table, pages = _layout(lens, 24)
+    cache = _cache(1, pages, 8, 24, 64, BF16)
+    pos = [p for n in lens for p in range(n)]
+    rows = [r for r, n in enumerate(lens) for _ in range(n)]
+    q, k, v = (torch.randn((len(pos), h, 64), device="cuda", dtype=BF16) for h in (32, 8, 8))
+    _check_append(cache, q, k, v, pos, table, paged.Rope.make(64), rows=rows)
+    _check_append(cache, q[:0], k[:0], v[:0], [], table, paged.Rope.make(64))
+
+
+def test_rope_matches_the_models_frequencies():
+    from cudallm_b200.synth import llama3_inv_freq
+    got = paged.Rope.make(64, scaling="llama3", scale=32.0).inv_freq.cpu().numpy()
+    assert np.allclose(got, llama3_inv_freq(), rtol=4 * EPS, atol=0)
+
+
+# ---- pages ------------------------------------------------------------------------------------
+
+def _check_fork(cache, tables, lens, refs, parents, room, out=None):
+    k0, v0 = _np(cache.k).copy(), _np(cache.v).copy()
+    inputs = [_ints(x) for x in (tables, lens, refs, parents)]
+    t, n, r, missing = cache.fork(*inputs, room=room, out=out)
+    want_t, want_n, want_r, want_missing, copies = R.fork_ref(np.array(tables), lens, np.array(refs), parents, cache.page_size, room)
+    for got, want in ((t, want_t), (n, want_n), (r, want_r), (missing, [want_missing])):
+        np.testing.assert_array_equal(_np(got), np.array(want))
+    for i, want in zip(inputs, (tables, lens, refs, parents)):
+        np.testing.assert_array_equal(_np(i), np.array(want))
+    for src, dst, tokens in copies:
+        k0[:, dst, :, :tokens], v0[:, dst, :, :tokens] = k0[:, src, :, :tokens], v0[:, src, :, :tokens]
+    np.testing.assert_array_equal(_np(cache.k), k0)
+    np.testing.assert_array_equal(_np(cache.v), v0)
+    return _np(t), _np(n), _np(r), int(missing)
+
+
+@pytest.mark.parametrize("order, kv_heads, dim, page", [("heads", 8, 64, 16), ("tokens", 2, 80, 5), ("heads", 1, 8, 1), ("tokens", 3, 256, 64)])
+def test_fork_walks_of_beams(order, kv_heads, dim, page):
+    """A prompt becomes beams, which branch, die and grow; the references stay those of the tables."""
+    rng = np.random.default_rng(page)
+    cache = _cache(3, 300 if page > 1 else 2000, kv_heads, page, dim, F16, order)
+    tables, lens, refs = (_np(x) for x in cache.rows(2, 40 if page > 1 else 200))
+    parents = [0, 1]
+    tables, lens, refs, missing = _check_fork(cache, tables, lens, refs, parents, 3 * page + 2)
+    assert missing == 0
+    lens = np.array([3 * page + 1, page], np.int32)
+    parents = [0, 0, 0, 0, 1, 1, 1, 1]
+    for step in range(12):
+        room = int(rng.integers(0, 3)) + (2 * page if step == 5 else 0)
+        tables, lens, refs, missing = _check_fork(cache, tables, lens, refs, parents, room)
+        assert missing == 0
+        held = tables[tables >= 0]
+        np.testing.assert_array_equal(np.bincount(held, minlength=cache.n_pages), refs)
+        lens = lens + min(room, 1)
+        parents = np.concatenate([rng.integers(0, 4, 4), rng.integers(4, 8, 4)])
+        if step % 4 == 3:
+            parents[rng.integers(0, 8)] = -1  # one sequence ends
+    tables, lens, refs, missing = _check_fork(cache, tables, lens, refs, [-1] * 3, 4)
+    assert not refs.any() and not lens.any() and (tables == -1).all()
+
+
+def test_fork_shared_tails_reserved_pages_and_references_of_others():
+    cache = _cache(2, 32, 2, 4, 64, BF16)
+    tables = [[3, 7, 9, 11, -1, -1], [3, 7, 9, -1, -1, -1], [20, -1, -1, -1, -1, -1], [-1, 5, 6, -1, 8, -1], [-1] * 6]
+    refs = np.zeros(32, np.int32)
+    for e in np.array(tables).ravel():
+        if e >= 0:
+            refs[e] += 1
+    refs[8] = 0    # after a gap: not the row's
+    refs[3] += 2   # held by someone else too
+    refs[20] += 1
+    lens = [9, 10, 4, 9, 0]
+    for parents in ([0, 1, 2, 3, 4], [4, 3, 2, 1, 0], [1, 1, 0], [3, 3, 3, 2, 2], [0, 0, 0, 5, -1, 99, 2 ** 31 - 1, -2 ** 31], []):
+        for room in (0, 1, 3, 4, 9):
+            _check_fork(cache, tables, lens, refs, parents, room)
+
+
+def test_fork_when_pages_run_out_or_the_table_ends():
+    cache = _cache(2, 6, 1, 4, 64, F16)
+    tables, lens, refs = [[0, 1, 2], [3, 4, -1]], [10, 7], np.array([1, 1, 1, 1, 1, 0], np.int32)
+    assert _check_fork(cache, tables, lens, refs, [0, 0, 0, 1, 1], 1)[3] == 2
+    assert _check_fork(cache, tables, lens, refs, [0, 1], 1)[3] == 0
+    assert _check_fork(cache, tables, lens, refs, [0, 1], 2 ** 31 - 1)[3] > 10 ** 8
+    assert _check_fork(cache, tables, [10 ** 9, -3], refs, [0, 1, 1], 0)[3] == 0
+    full = np.ones(6, np.int32)
+    assert _check_fork(cache, tables, lens, full, [0, 0], 0)[3] == 1
+    assert _check_fork(cache, tables, lens, refs, [-1, -1], 5)[3] == 0
+
+
+def test_fork_many_rows_and_pages():
+    rng = np.random.default_rng(5)
+    rows, page, pages = 1500, 4, 9000
+    lens = rng.integers(0, 20, rows)
+    table, _ = _layout(list(lens), page, width=8)
+    refs = np.bincount(table[table >= 0], minlength=pages).astype(np.int32)
+    cache = _cache(1, pages, 1, page, 8, F16)
+    _check_fork(cache, table, lens, refs, rng.integers(-1, rows, 2500), 2)
+    _check_fork(cache, table, lens, refs, rng.integers(0, 3, 30), 2)
+
+
+def test_fork_into_the_other_half_of_a_pair():
+    cache = _cache(1, 64, 2, 16, 64, F16)
+    tables, lens, refs = cache.rows(4, 4)
+    other = (*(torch.full_like(x, 77) for x in (tables, lens, refs)), torch.full((1,), 77, dtype=torch.int32, device="cuda"))
+    state = cache.fork(tables, lens, refs, _ints([0, 1, 2, 3]), room=20, out=other)
+    assert state is other and _np(state[2]).sum() == 8 and int(state[3]) == 0
+    with pytest.raises(CudaLLMError, match="overlap"):
+        cache.fork(*state[:3], _ints([0, 1, 2, 3]), out=state)
+
+
+@pytest.mark.parametrize("order", ["heads", "tokens"])
+@pytest.mark.parametrize("pages, share", [(1, 1.0), (7, 0.5), (500, 0.0), (500, 0.02), (500, 0.5), (500, 0.97), (500, 1.0), (3000, 0.3)])
+def test_compact(pages, share, order):
+    rng = np.random.default_rng(pages)
+    cache = _cache(2, pages, 2, 4, 64, F16, order)
+    used = np.nonzero(rng.random(pages) < share)[0]
+    tables = rng.choice(np.concatenate([used, [-1, -5, pages, 2 ** 31 - 1]]), (5, 40)).astype(np.int32)
+    refs = np.zeros(pages, np.int32)
+    refs[used] = rng.integers(1, 5, len(used))
+    k0, v0 = _np(cache.k).copy(), _np(cache.v).copy()
+    t, r, live = cache.compact(_ints(tables), _ints(refs))
+    want_t, want_r, want_live, moves = R.compact_ref(tables, refs)
+    np.testing.assert_array_equal(_np(t), want_t)
+    np.testing.assert_array_equal(_np(r), want_r)
+    assert int(live) == want_live
+    for src, dst in moves:
+        k0[:, dst], v0[:, dst] = k0[:, src], v0[:, src]
+    np.testing.assert_array_equal(_np(cache.k), k0)
+    np.testing.assert_array_equal(_np(cache.v), v0)
+
+
+def test_compact_keeps_attention():
+    lens = [100, 37, 200]
+    table, pages = _layout(lens, 16, spare=40)
+    cache = _cache(1, pages, 2, 16, 64, F16)
+    q = torch.randn((3, 8, 64), device="cuda")
+    before = cache.attend(q, _ints(table), _ints(lens))
+    refs = np.bincount(table[table >= 0], minlength=pages).astype(np.int32)
+    t, r, live = cache.compact(_ints(table), _ints(refs))
+    assert int(t.max()) < int(live)
+    assert torch.equal(cache.attend(q, t, _ints(lens)), before)
+
+
+# ---- selection --------------------------------------------------------------------------------
+
+def _check_beam(logits, scores, keep, finished=None, eos=0):
+    got = paged.beam_select(logits, _f32(scores), keep=keep, finished=None if finished is None else _ints(finished), eos=eos)
+    x = _np(logits)
+    ref, parents, tokens = R.beam_ref(x, np.array(scores, np.float32).astype(np.float64), keep, finished, eos)
+    np.testing.assert_array_equal(_np(got[1]), parents)
+    np.testing.assert_array_equal(_np(got[2]), tokens)
+    big = np.abs(x[np.isfinite(x)]).max(initial=0.0) + np.log(x.shape[1]) + np.sqrt(x.shape[1])
+    _within(got[0], ref, 8 * EPS * (np.abs(np.where(np.isfinite(ref), ref, 0)) + 2 * big))
+
+
+def _f32(a):
+    return torch.from_numpy(np.array(a, np.float32)).cuda()
+
+
+@pytest.mark.parametrize("x", [F32, F16, BF16])
+@pytest.mark.parametrize("groups, beams, keep, vocab", [(1, 1, 1, 1), (1, 4, 8, 1000), (3, 5, 5, 32007), (2, 1, 64, 128256), (1, 64, 64, 4099), (2, 8, 16, 128256),
+                                                        (4, 3, 7, 50), (1, 2, 6, 3), (1, 64, 64, 1), (5, 4, 1, 257)])
+def test_beam_sizes(x, groups, beams, keep, vocab):
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    logits = (3 * torch.randn((groups * beams, vocab), generator=gen, device="cuda")).to(x)
+    scores = np.random.default_rng(vocab).normal(-5, 2, (groups, beams))
+    _check_beam(logits, scores, keep)
+
+
+@pytest.mark.parametrize("vocab", [5, 900, 70001])
+def test_beam_ties_go_to_the_lower_row_then_token(vocab):
+    keep = 9
+    same = torch.zeros((4, vocab), device="cuda")
+    _check_beam(same, [[0.0, 0.0, 0.0, 0.0]], keep)
+    _check_beam(same, [[-1.0, 0.0, 0.0, -1.0]], keep)
+    _check_beam(-same, [[-2.0, -2.0, -2.0, -2.0]], keep)
+    few = torch.randint(0, 3, (4, vocab), device="cuda").to(BF16)
+    few[1:] = few[0]
+    few[2, ::2] *= -1.0  # zeros of both signs are equal
+    few[2] = few[2].abs()
+    _check_beam(few, [[-1.0, -1.0, -1.0, -1.0]], keep)
+
+
+def test_beam_equal_zeros():
+    x = torch.zeros((1, 300), device="cuda")
+    x[0, ::3] = -0.0
+    _check_beam(x, [[0.0]], 8)
+
+
+def test_beam_rising_and_falling_rows():
+    up = torch.arange(50000, device="cuda", dtype=torch.float32) / 5000
+    _check_beam(torch.stack([up, up.flip(0)]), [[-1.0, -1.2]], 33)
+
+
+def test_beam_masked_and_poisoned_rows():
+    inf = float("inf")
+    x = torch.randn((6, 5000), device="cuda")
+    x[0] = -inf                     # nothing left
+    x[1, 10:] = -inf                # fewer tokens than are kept
+    x[2, 77] = float("nan")         # a row that is not a number
+    x[3, 5] = inf
+    x[4, :2500] = torch.finfo(F32).min
+    scores = [[-1.0, -1.0, -1.0, -1.0, -1.0, -30.0]]
+    _check_beam(x, scores, 20)
+    _check_beam(x, [[-1.0, -1.0, -1.0, -1.0, -inf, float("nan")]], 20)
+    _check_beam(x[:1], [[0.0]], 5)
+    _check_beam(x[2:3], [[0.0]], 5)
+    _check_beam(x[3:4], [[0.0]], 5)
+    _check_beam(torch.full((2, 3000), -inf, device="cuda"), [[-inf, 0.0]], 4)
+
+
+def test_beam_finished_rows():
+    x = torch.randn((8, 3000), device="cuda")
+    x[3] = float("nan")  # a finished beam's row is not read
+    scores = np.random.default_rng(1).normal(-3, 1, (2, 4))
+    _check_beam(x, scores, 8, finished=[[1, 0, 0, 1], [0, 0, 0, 0]], eos=2999)
+    _check_beam(x, scores, 8, finished=[[1, 1, 1, 1], [1, 1, 0, 2]], eos=0)
+
+
+def test_beam_strided_and_shared_rows():
+    wide = torch.randn((8, 1101), device="cuda", dtype=BF16)
+    _check_beam(wide[:, 1:1001], [[-1.0] * 4, [-2.0] * 4], 5)
+    _check_beam(wide[::2, 3:1000], [[-1.0] * 4], 5)
+    _check_beam(wide[:1].expand(4, 1101), [[-1.0, -1.5, -2.0, -2.5]], 8)
+
+
+def test_beam_same_bits_in_a_graph_and_on_two_streams():
+    x, s = torch.randn((16, 128256), device="cuda"), _f32(np.random.default_rng(2).normal(-5, 1, (4, 4)))
+    ref = paged.beam_select(x, s, keep=8)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        there = [paged.beam_select(x, s, keep=8) for _ in range(10)]
+    here = [paged.beam_select(x, s, keep=8) for _ in range(10)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged.beam_select(x, s, keep=8)
+    graph.replay()
+    torch.cuda.synchronize()
+    for got in there + here + [out]:
+        assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+# ---- refusals ---------------------------------------------------------------------------------
+
+def test_refusals():
+    cache = _cache(2, 8, 2, 16, 64, F16)
+    t, n, r = cache.rows(2, 3)
+    q, k = torch.zeros((2, 8, 64), device="cuda"), torch.zeros((2, 2, 64), device="cuda")
+    rope = paged.Rope.make(64)
+    pos = _ints([0, 0])
+    bad = [
+        lambda: cache.attend(q, t, n, layer=2),
+        lambda: cache.attend(q, t, n, layer=-1),
+        lambda: cache.attend(q[:, :5], t, n),                     # 5 heads for 2 key heads
+        lambda: cache.attend(q[:, :, :32], t, n),
+        lambda: cache.attend(q.double(), t, n),
+        lambda: cache.attend(q.cpu(), t, n),
+        lambda: cache.attend(q, t[:1], n),
+        lambda: cache.attend(q, t.long(), n),
+        lambda: cache.attend(q, t, n[:1]),
+        lambda: cache.attend(q, t, n, window=-1),
+        lambda: cache.attend(q, t, n, scale=float("nan")),
+        lambda: cache.attend(q, t, n, out=q),
+        lambda: cache.attend(q, t, n, out=q.half()),
+        lambda: cache.attend(q.transpose(1, 2).contiguous().transpose(1, 2), t, n),
+        lambda: cache.append(q, k[:1], k, pos, t, rope),
+        lambda: cache.append(q, k, k.half(), pos, t, rope),
+        lambda: cache.append(q, k[:, :1], k[:, :1], pos, t, rope),
+        lambda: cache.append(q, k, k, pos.long(), t, rope),
+        lambda: cache.append(q, k, k, pos, t, paged.Rope.make(128)),
+        lambda: cache.append(q, k, k, pos, t, rope, layer=2),
+        lambda: cache.append(q[:, :7], k, k, pos, t, rope, out=q[:, 1:]),  # neither q itself nor apart from it
+        lambda: cache.append(q, k, k, pos, t, rope, out=q[:1, :1].expand(2, 8, 64)),
+        lambda: cache.fork(t, n, r[:4], pos),
+        lambda: cache.fork(t, n, r, pos, room=-1),
+        lambda: cache.fork(t, n, r, pos.long()),
+        lambda: cache.fork(t, n, r, pos, out=(t, n.clone(), r.clone(), pos[:1].clone())),
+        lambda: cache.compact(t, r, out=(t.clone(), r, pos[:1].clone())),
+        lambda: cache.compact(t, r.long()),
+        lambda: paged.beam_select(q[0], _f32([[0.0] * 8]), keep=0),
+        lambda: paged.beam_select(q[0], _f32([[0.0] * 8]), keep=65),
+        lambda: paged.beam_select(q[0], _f32([[0.0] * 7]), keep=1),
+        lambda: paged.beam_select(q[0, :, :1], _f32([[0.0] * 8]), keep=9),
+        lambda: paged.beam_select(q[0], _f32([[0.0] * 8]), keep=1, finished=_ints([[0] * 8]), eos=64),
+        lambda: paged.beam_select(q[0].double(), _f32([[0.0] * 8]), keep=1),
+        lambda: paged.PagedCache(cache.k, cache.v[:, :, :, :8]),
+        lambda: paged.PagedCache(cache.k.float(), cache.v.float()),
+        lambda: paged.PagedCache(cache.k[..., :60], cache.v[..., :60]),
+        lambda: paged.PagedCache(cache.k.transpose(3, 4), cache.v.transpose(3, 4)),
+        lambda: paged.PagedCache(cache.k[:1].expand(2, -1, -1, -1, -1), cache.v[:1].expand(2, -1, -1, -1, -1)).attend(q, t, n),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(CudaLLMError) as e:
+            call()
+        assert e.value.code == 1, i
+    torch.cuda.synchronize()

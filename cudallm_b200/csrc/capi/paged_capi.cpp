@@ -111,7 +111,7 @@ int cudallm_paged_attend(const cudallm_pages* pages, const cudallm_attend_args* 
         if (a->n_seq == 0) return;
         CLLM_REQUIRE(a->n_heads > 0 && a->n_heads % pages->n_kv_heads == 0, "n_heads must be a positive multiple of n_kv_heads");
         CLLM_REQUIRE(static_cast<long long>(a->n_seq) * a->n_heads <= INT_MAX, "n_seq * n_heads must be below 2^31");
-        CLLM_REQUIRE(static_cast<long long>(a->table_width) * pages->page_size <= INT_MAX, "a row must hold fewer than 2^31 tokens");
+        CLLM_REQUIRE(static_cast<long long>(a->table_width) * pages->page_size <= INT_MAX - 64, "a row must hold fewer than 2^31 - 64 tokens");
         CLLM_REQUIRE(a->window >= 0 && std::isfinite(a->scale), "window must not be negative, scale must be finite");
         const size_t es = x_bytes(a->x_dtype);
         CLLM_REQUIRE(a->q != nullptr && a->lens != nullptr && a->out != nullptr, "q, lens and out must be non-null");

@@ -3,107 +3,696 @@
 //   out[b][h] = sum_t exp(s_t - m) v_t / sum_t exp(s_t - m),  s_t = scale q.k_t,  m = max_t s_t,
 //   lse[b][h] = m + ln sum_t exp(s_t - m)
 //
-// One block per (sequence, query head); each warp takes every fourth position, lanes hold the head's dims, and the
-// warps' running (m, sum, out) are merged in warp order.
-#include <climits>
+// What bounds it: every key and value is read once (2 tokens kv_heads head_dim 2 B) for 4 flops per query head of
+// its group and element, so HBM does for groups of up to 16 heads.
+//
+// Split. The positions of all (sequence, key head) items are cut into tiles of kTile tokens and counted through from
+// first to last; CTA c takes tiles [c Q, (c + 1) Q), so ragged lengths spread evenly and one long sequence covers the
+// GPU. A CTA's part of an item is a segment; the warps of the CTA take its tiles in turn, each with its own running (m,
+// sum, out), which are joined in warp order. Segments that are not a whole item are left in the workspace, and the
+// last CTA of the item to arrive joins them in order: no result depends on the order of arrival.
+//
+// Tiles. A warp copies its tiles with 16-byte asynchronous copies into a ring of its own (no block barrier between
+// tiles), three deep; each lane looks up the page of one token, so pages of any size may end inside a tile. Rows are
+// swizzled (chunk ^ row % 8) so that ldmatrix reads them without bank conflicts. Tokens without a page, outside the
+// window or past the length are filled with zeros instead of being read, and masked by one bit each.
+//
+// Arithmetic. m16n8k16 matrix instructions with fp32 accumulators, 8 query heads a group: the second 8 rows of the
+// 16-row operand are free, so they carry a second plane of it. Scores: q as one plane of the cache's type when it has
+// that type, else as its rounding and the rounding of the rest (fp16: 22 bits; bf16: a third plane makes 24 bits for
+// fp32 queries). Weights: p likewise in two planes (three for fp32 results over bf16), so that rounding p never shows
+// in the result. Each tile's product starts from zero and is added to the running fp32 output outside of the
+// tensor core, whose additions truncate.
+#include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstring>
 
 #include "common/check.h"
+#include "kernels/kernels.h"
 #include "kernels/paged.h"
 #include "kernels/paged_common.cuh"
+#include "kernels/ptx.cuh"
 
 namespace cudallm {
 
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kDimsPerLane = 8;  // 256 / 32
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStages = 3;
+constexpr int kMaxCtas = 512;
+constexpr int kMaxRows = 2048;          // sequences of one launch (their tile counts are summed in shared memory)
+constexpr int kSlotFloats = 16 * 2 + 16 * 128;  // a partial: m, sum and out of 16 heads x 128 dims or 8 x 256
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-template <typename X, typename KV>
-__global__ void __launch_bounds__(32 * kWarps) attend_kernel(cudallm_pages pg, cudallm_attend_args a) {
-    __shared__ float sm_m[kWarps], sm_l[kWarps], sm_o[kWarps][256];
-    const int b = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads;
-    const int kvh = h / (a.n_heads / pg.n_kv_heads);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = pg.head_dim;
-    const long long cap = static_cast<long long>(a.table_width) * pg.page_size;
-    const int len = static_cast<int>(min(static_cast<long long>(max(a.lens[b], 0)), cap));
-    const int first = a.window > 0 ? max(0, len - a.window) : 0;
-    const X* q = static_cast<const X*>(a.q) + b * a.q_seq_stride + h * a.q_head_stride;
-    const KV* K = static_cast<const KV*>(pg.k) + a.layer * pg.layer_stride + kvh * pg.head_stride;
-    const KV* V = static_cast<const KV*>(pg.v) + a.layer * pg.layer_stride + kvh * pg.head_stride;
-    float qv[kDimsPerLane], o[kDimsPerLane], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < kDimsPerLane; ++i) {
-        const int d = lane + 32 * i;
-        qv[i] = d < hd ? as_float(q[d]) * a.scale : 0.f;
-        o[i] = 0.f;
-    }
-    for (int t = first + warp; t < len; t += kWarps) {
-        const int page = a.tables[b * a.table_stride + t / pg.page_size];
-        if (page < 0 || page >= pg.n_pages) continue;
-        const long long at = page * pg.page_stride + (t % pg.page_size) * pg.token_stride;
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < kDimsPerLane; ++i) {
-            const int d = lane + 32 * i;
-            if (d < hd) s = fmaf(qv[i], as_float(K[at + d]), s);
-        }
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        const float mn = fmaxf(m, s), old = expf(m - mn), p = expf(s - mn);
-        m = mn;
-        l = l * old + p;
-#pragma unroll
-        for (int i = 0; i < kDimsPerLane; ++i) {
-            const int d = lane + 32 * i;
-            if (d < hd) o[i] = fmaf(p, as_float(V[at + d]), o[i] * old);
-        }
-    }
-    if (lane == 0) {
-        sm_m[warp] = m;
-        sm_l[warp] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < kDimsPerLane; ++i) sm_o[warp][lane + 32 * i] = o[i];
-    __syncthreads();
-    float mm = -INFINITY, ll = 0.f;
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, sm_m[w]);
-    float scale[kWarps];
-    for (int w = 0; w < kWarps; ++w) {
-        scale[w] = mm == -INFINITY ? 0.f : expf(sm_m[w] - mm);
-        ll += scale[w] * sm_l[w];
-    }
-    X* out = static_cast<X*>(a.out) + static_cast<long long>(blockIdx.x) * hd;
-    for (int d = threadIdx.x; d < hd; d += blockDim.x) {
-        float v = 0.f;
-        for (int w = 0; w < kWarps; ++w) v += scale[w] * sm_o[w][d];
-        out[d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
-    }
-    if (a.lse != nullptr && threadIdx.x == 0) a.lse[blockIdx.x] = mm + logf(ll);
+// n / d for 0 <= n < 2^31 as a multiplication.
+struct FastDiv {
+    unsigned mul, shift;
+};
+FastDiv fast_div(int d) {
+    unsigned s = 0;
+    while ((1u << s) < static_cast<unsigned>(d)) ++s;
+    return {static_cast<unsigned>(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+}
+__device__ __forceinline__ int div_by(int n, FastDiv f) {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(n)) * f.mul) >> f.shift);
 }
 
-template <typename X>
-void launch_for(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStream_t stream) {
-    const unsigned grid = static_cast<unsigned>(a.n_seq) * a.n_heads;
-    if (pg.kv_dtype == CUDALLM_KV_BF16) {
-        attend_kernel<X, __nv_bfloat16><<<grid, 32 * kWarps, 0, stream>>>(pg, a);
+struct Params {
+    const void* q;
+    const char* k;  // the layer's pages
+    const char* v;
+    void* out;
+    float* lse;
+    const int* tables;
+    const int* lens;
+    float* parts;       // [CTA][2] partials
+    unsigned* arrived;  // [CTA]
+    long long q_seq_stride, q_head_stride, table_stride, page_stride, head_stride, token_stride;  // elements
+    float scale2;                                                                                  // scale * log2(e)
+    int n_seq, n_heads, n_pages, page_size, table_width, head_dim, window;
+    int group;      // query heads per key head
+    int per_head;   // items per key head (groups of 8 HG query heads)
+    int items;      // items per sequence
+    FastDiv page_div;
+};
+
+template <typename KV>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                   uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// 16 bytes global -> shared, or 16 zero bytes where `bytes` is 0.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// (a, b) rounded to the cache's type and packed, a in the low half; a and b keep what the rounding left.
+template <typename KV>
+__device__ __forceinline__ uint32_t take_plane(float& a, float& b) {
+    const KV ha = from_float<KV>(a), hb = from_float<KV>(b);
+    a -= as_float(ha);
+    b -= as_float(hb);
+    uint16_t ua, ub;
+    memcpy(&ua, &ha, 2);
+    memcpy(&ub, &hb, 2);
+    return static_cast<uint32_t>(ub) << 16 | ua;
+}
+
+template <typename A, typename B>
+struct Same {
+    static constexpr bool value = false;
+};
+template <typename A>
+struct Same<A, A> {
+    static constexpr bool value = true;
+};
+
+// HD: head dims rounded up to 64, 128 or 256; HG: groups of 8 query heads of an item.
+template <typename X, typename KV, int HD, int HG>
+struct Shape {
+    static constexpr bool kBf16 = Same<KV, __nv_bfloat16>::value, kF32 = Same<X, float>::value;
+    static constexpr int kQPlanes = Same<X, KV>::value ? 1 : kBf16 && kF32 ? 3 : 2;
+    static constexpr int kPPlanes = kBf16 && kF32 ? 3 : 2;
+    static constexpr int kTile = HD == 64 ? 32 : 16;  // tokens
+    static constexpr int kRowBytes = HD * 2;
+    static constexpr int kPlaneBytes = kTile * kRowBytes;  // keys or values of a tile
+    static constexpr int kStageBytes = 2 * kPlaneBytes;
+    static constexpr int kHeads = 8 * HG;
+    static constexpr int kRing = kWarps * kStages * kStageBytes;
+    static constexpr int kMerge = kWarps * 8 * (64 + 2) * 4;  // the warps' results of 8 heads x 64 dims
+    static constexpr int kFixed = kRing + kMerge + kWarps * kStages * 4 + 64;
+};
+
+struct Segment {
+    int b, item;       // sequence, item of it
+    int t0, t1, tiles;  // [t0, t1) of the item's tiles
+    unsigned at;       // flat number of the item's first tile
+    int first_tile;    // of the sequence: where the window starts
+};
+
+// One CTA's walk over its flat range of tiles.
+struct Walk {
+    const unsigned* before;  // [n_seq + 1] flat tiles of one item before sequence b (shared memory)
+    int n_seq, items, pad;   // items per sequence; tiles of an item are rounded up to `pad` in the flat count
+    unsigned f1;             // end of this CTA's range
+};
+
+template <int TILE>
+__device__ __forceinline__ void tiles_of(const Params& p, int b, int& len, int& first, int& first_tile, int& tiles) {
+    const int cap = p.table_width * p.page_size;  // below 2^31 (checked on the host)
+    len = min(max(p.lens[b], 0), cap);
+    first = p.window > 0 ? max(0, len - p.window) : 0;
+    first_tile = first / TILE;
+    tiles = len > 0 ? (len + TILE - 1) / TILE - first_tile : 0;
+}
+
+// The segment of sequence b, item `item` from flat tile f on.
+template <int TILE>
+__device__ __forceinline__ void open_segment(const Params& p, const Walk& w, Segment& s, int b, int item, unsigned f) {
+    int len, first;
+    s.b = b;
+    s.item = item;
+    tiles_of<TILE>(p, b, len, first, s.first_tile, s.tiles);
+    const unsigned padded = w.before[b + 1] - w.before[b];
+    s.at = w.before[b] * w.items + item * padded;
+    s.t0 = static_cast<int>(f - s.at);
+    s.t1 = static_cast<int>(min(static_cast<unsigned>(s.tiles), w.f1 - s.at));
+}
+
+// The next segment; false when the range is done.
+template <int TILE>
+__device__ __forceinline__ bool next_segment(const Params& p, const Walk& w, Segment& s) {
+    const unsigned padded = w.before[s.b + 1] - w.before[s.b];
+    const unsigned f = s.at + padded;  // where the next item starts
+    if (f >= w.f1) return false;
+    int b = s.b, item = s.item + 1;
+    if (item == w.items) {
+        item = 0;
+        do ++b;
+        while (w.before[b + 1] == w.before[b]);
+    }
+    open_segment<TILE>(p, w, s, b, item, f);
+    return true;
+}
+
+template <typename X, typename KV, int HD, int HG>
+__global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ Params p) {
+    using S = Shape<X, KV, HD, HG>;
+    constexpr int TILE = S::kTile, NT = TILE / 8, KS = HD / 16, JS = TILE / 16;
+    extern __shared__ __align__(128) char smem[];
+    char* ring = smem;
+    float* merge_o = reinterpret_cast<float*>(smem + S::kRing);  // [warp][8 heads][64 dims]
+    float* merge_m = merge_o + kWarps * 8 * 64;                  // [warp][8]
+    float* merge_l = merge_m + kWarps * 8;
+    unsigned* masks = reinterpret_cast<unsigned*>(merge_l + kWarps * 8);  // [warp][stage]
+    unsigned* shared_word = masks + kWarps * kStages;                     // [16]
+    unsigned* before = reinterpret_cast<unsigned*>(smem + S::kFixed);     // [n_seq + 1]
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int g = lane >> 2, t4 = lane & 3, hd = p.head_dim;
+
+    // Tiles of one item before each sequence, as they are and rounded up to kWarps; empty rows are answered here.
+    unsigned total = 0, total_pad = 0;
+    for (int b0 = 0; b0 < p.n_seq; b0 += kThreads) {
+        const int b = b0 + threadIdx.x;
+        int len, first, first_tile, tiles = 0;
+        if (b < p.n_seq) tiles_of<TILE>(p, b, len, first, first_tile, tiles);
+        unsigned s = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned t = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += t;
+        }
+        const unsigned pads = __reduce_add_sync(0xffffffffu, (tiles + kWarps - 1) / kWarps);
+        if (lane == 31) {
+            shared_word[warp] = s;
+            shared_word[kWarps + warp] = pads;
+        }
+        __syncthreads();
+        unsigned base = total;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) base += shared_word[w];
+            total += shared_word[w];
+            total_pad += shared_word[kWarps + w];
+        }
+        if (b < p.n_seq) before[b] = base + s - tiles;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) before[p.n_seq] = total;
+    for (int b = blockIdx.x; b < p.n_seq; b += gridDim.x) {
+        if (p.lens[b] > 0 && p.table_width > 0) continue;
+        for (int i = threadIdx.x; i < p.n_heads * hd; i += kThreads) {
+            static_cast<X*>(p.out)[static_cast<long long>(b) * p.n_heads * hd + i] = from_float<X>(0.f);
+        }
+        if (p.lse != nullptr) {
+            for (int h = threadIdx.x; h < p.n_heads; h += kThreads) p.lse[static_cast<long long>(b) * p.n_heads + h] = -INFINITY;
+        }
+    }
+    // Few tiles: an item's tiles are cut every kWarps, one tile a warp. Otherwise every CTA takes an equal share.
+    const bool few = total_pad * p.items <= gridDim.x;
+    const unsigned share = few ? kWarps : (total * p.items + gridDim.x - 1) / gridDim.x;
+    const unsigned all = few ? total_pad * kWarps * p.items : total * p.items;
+    __syncthreads();
+    if (few) {  // the same sums of rounded tile counts
+        unsigned run = 0;
+        for (int b0 = 0; b0 < p.n_seq; b0 += kThreads) {
+            const int b = b0 + threadIdx.x;
+            const unsigned mine = b < p.n_seq ? (before[b + 1] - before[b] + kWarps - 1) / kWarps * kWarps : 0;
+            unsigned s = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const unsigned t = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += t;
+            }
+            if (lane == 31) shared_word[warp] = s;
+            __syncthreads();
+            unsigned base = run;
+            for (int w = 0; w < kWarps; ++w) {
+                if (w < warp) base += shared_word[w];
+                run += shared_word[w];
+            }
+            if (b < p.n_seq) before[b] = base + s - mine;
+            __syncthreads();
+        }
+        if (threadIdx.x == 0) before[p.n_seq] = run;
+        __syncthreads();
+    }
+    const unsigned f0 = min(all, blockIdx.x * share);
+    Walk walk{before, p.n_seq, p.items, few ? kWarps : 1, min(all, f0 + share)};
+    if (f0 >= walk.f1) return;
+
+    // The first segment: the last sequence that starts at or before f0.
+    Segment seg;
+    {
+        int lo = 0, hi = p.n_seq;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (before[mid] * p.items <= f0) lo = mid;
+            else hi = mid;
+        }
+        const unsigned padded = before[lo + 1] - before[lo];
+        open_segment<TILE>(p, walk, seg, lo, static_cast<int>((f0 - before[lo] * p.items) / padded), f0);
+    }
+
+    // ---- the warp's stream of tiles ----
+    Segment ls = seg;                  // of the next tile to load
+    int lt = ls.t0 + warp;             // that tile
+    bool more = true;                  // there is one
+    int l_slot = 0, l_token = 0;       // this lane's token of it, and its slot in its page
+    int l_page = -1;
+    bool l_valid = false;
+    const uint32_t my_ring = smem_addr(ring) + warp * (kStages * S::kStageBytes);
+    auto look_up = [&] {  // moves to the next tile of this warp and reads its lane's page number
+        while (more && lt >= ls.t1) {
+            more = next_segment<TILE>(p, walk, ls);
+            lt = ls.t0 + warp;
+        }
+        if (!more) return;
+        int len, first, ft, tiles;
+        tiles_of<TILE>(p, ls.b, len, first, ft, tiles);
+        l_token = (ls.first_tile + lt) * TILE + (lane % TILE);
+        l_valid = l_token >= first && l_token < len;
+        const int entry = div_by(l_token, p.page_div);
+        l_slot = l_token - entry * p.page_size;
+        l_page = l_valid ? p.tables[ls.b * p.table_stride + entry] : -1;
+    };
+    auto load_tile = [&](int stage) {
+        if (more) {
+            const bool valid = l_page >= 0 && l_page < p.n_pages;
+            const long long off = valid ? (l_page * p.page_stride + l_slot * p.token_stride + ls.item / p.per_head * p.head_stride) * 2 : -1;
+            const unsigned mask = __ballot_sync(0xffffffffu, valid);
+            if (lane == 0) masks[warp * kStages + stage] = mask;
+            constexpr int kChunks = HD / 8, kRowsAtOnce = 32 / (kChunks < 32 ? kChunks : 32);
+            const int c = lane % kChunks;
+            const bool inside = c * 8 < hd;
+            const uint32_t dst = my_ring + stage * S::kStageBytes;
+#pragma unroll
+            for (int r0 = 0; r0 < TILE; r0 += kRowsAtOnce) {
+                const int r = r0 + lane / kChunks;
+                const long long o = __shfl_sync(0xffffffffu, off, r);
+                const int bytes = o >= 0 && inside ? 16 : 0;
+                const long long at = bytes ? o + c * 16 : 0;
+                const uint32_t d = dst + r * S::kRowBytes + ((c ^ (r & 7)) << 4);
+                copy16(d, p.k + at, bytes);
+                copy16(d + S::kPlaneBytes, p.v + at, bytes);
+            }
+            lt += kWarps;
+        }
+        copy_commit();
+    };
+    look_up();
+#pragma unroll
+    for (int s = 0; s < kStages - 1; ++s) {
+        load_tile(s);
+        look_up();
+    }
+
+    int stage = 0;
+    for (;;) {
+        // ---- one segment ----
+        const int kvh = seg.item / p.per_head, h_first = (seg.item % p.per_head) * S::kHeads;
+        const int heads = min(S::kHeads, p.group - h_first);  // query heads of this item
+        const long long row0 = static_cast<long long>(seg.b) * p.n_heads + kvh * p.group + h_first;
+
+        uint32_t qf[HG][KS][S::kQPlanes][2];  // planes of q: dims 16 ks + 2 t4 + {0, 1} and + 8
+        float q_scale[HG];
+#pragma unroll
+        for (int hg = 0; hg < HG; ++hg) {
+            const int h = hg * 8 + g;
+            const X* q = static_cast<const X*>(p.q) + seg.b * p.q_seq_stride + (kvh * p.group + h_first + h) * p.q_head_stride;
+            float raw[KS][4];
+            float top = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = ks * 16 + 2 * t4 + (e & 1) + (e >> 1) * 8;
+                    raw[ks][e] = h < heads && d < hd ? as_float(q[d]) : 0.f;
+                    top = fmaxf(top, fabsf(raw[ks][e]));
+                }
+            }
+            q_scale[hg] = p.scale2;
+            float shrink = 1.f;
+            if constexpr (!S::kBf16 && S::kQPlanes > 1) {
+                // fp16 planes: the head is brought to 1 <= max|q| < 2 by a power of two, which the scale gives back.
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253) - 127;
+                shrink = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                q_scale[hg] *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = raw[ks][e] * shrink;
+#pragma unroll
+                for (int pl = 0; pl < S::kQPlanes; ++pl) {
+                    qf[hg][ks][pl][0] = take_plane<KV>(v[0], v[1]);
+                    qf[hg][ks][pl][1] = take_plane<KV>(v[2], v[3]);
+                }
+            }
+        }
+
+        float o[HG][HD / 8][2], m[HG], l[HG];
+#pragma unroll
+        for (int hg = 0; hg < HG; ++hg) {
+            m[hg] = -INFINITY;
+            l[hg] = 0.f;
+#pragma unroll
+            for (int n = 0; n < HD / 8; ++n) o[hg][n][0] = o[hg][n][1] = 0.f;
+        }
+
+        for (int t = seg.t0 + warp; t < seg.t1; t += kWarps) {
+            load_tile(stage == 0 ? kStages - 1 : stage - 1);
+            look_up();
+            copy_wait<kStages - 1>();
+            __syncwarp();
+            const uint32_t kb = my_ring + stage * S::kStageBytes, vb = kb + S::kPlaneBytes;
+            const unsigned mask = masks[warp * kStages + stage];
+
+            // scores
+            float s[HG][NT][4];
+#pragma unroll
+            for (int hg = 0; hg < HG; ++hg)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[hg][n][e] = 0.f;
+            const int k_row = (lane >> 4) * 8 + (lane & 7), k_chunk = (lane >> 3) & 1;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                if (ks * 16 >= hd) break;
+#pragma unroll
+                for (int n2 = 0; n2 < NT / 2; ++n2) {
+                    const int r = n2 * 16 + k_row;
+                    uint32_t b[4];
+                    ldmatrix4(b, kb + r * S::kRowBytes + (((2 * ks + k_chunk) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int hg = 0; hg < HG; ++hg) {
+                        const uint32_t lo0 = S::kQPlanes > 1 ? qf[hg][ks][S::kQPlanes > 1][0] : 0u;
+                        const uint32_t lo1 = S::kQPlanes > 1 ? qf[hg][ks][S::kQPlanes > 1][1] : 0u;
+                        mma<KV>(s[hg][2 * n2], qf[hg][ks][0][0], lo0, qf[hg][ks][0][1], lo1, b[0], b[1]);
+                        mma<KV>(s[hg][2 * n2 + 1], qf[hg][ks][0][0], lo0, qf[hg][ks][0][1], lo1, b[2], b[3]);
+                        if constexpr (S::kQPlanes > 2) {
+                            mma<KV>(s[hg][2 * n2], qf[hg][ks][2][0], 0u, qf[hg][ks][2][1], 0u, b[0], b[1]);
+                            mma<KV>(s[hg][2 * n2 + 1], qf[hg][ks][2][0], 0u, qf[hg][ks][2][1], 0u, b[2], b[3]);
+                        }
+                    }
+                }
+            }
+
+            // weights: this thread has tokens 8 n + 2 t4 + {0, 1} of head g
+            constexpr unsigned kAll = TILE == 32 ? 0xffffffffu : 0xffffu;
+            const bool whole = (mask & kAll) == kAll;
+            uint32_t pf[HG][JS][S::kPPlanes][2];
+            float fade[HG];
+#pragma unroll
+            for (int hg = 0; hg < HG; ++hg) {
+                float x[NT][2], top = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        x[n][e] = (s[hg][n][e] + s[hg][n][2 + e]) * q_scale[hg];
+                        if (!whole && !((mask >> (8 * n + 2 * t4 + e)) & 1u)) x[n][e] = -INFINITY;
+                        top = fmaxf(top, x[n][e]);
+                    }
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float m_new = fmaxf(m[hg], top), ref = m_new == -INFINITY ? 0.f : m_new;
+                fade[hg] = exp2f(m[hg] - ref);
+                m[hg] = m_new;
+                float sum = 0.f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        x[n][e] = exp2f(x[n][e] - ref);
+                        sum += x[n][e];
+                    }
+                }
+                l[hg] = l[hg] * fade[hg] + sum;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int pl = 0; pl < S::kPPlanes; ++pl) pf[hg][n / 2][pl][n & 1] = take_plane<KV>(x[n][0], x[n][1]);
+            }
+
+            // out = out * fade + weights x values
+            const int v_row = lane & 15, v_chunk = lane >> 4;
+#pragma unroll
+            for (int n2 = 0; n2 < HD / 16; ++n2) {
+                if (n2 * 16 >= hd) break;
+                float acc[HG][2][4];
+#pragma unroll
+                for (int hg = 0; hg < HG; ++hg)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[hg][i][e] = 0.f;
+#pragma unroll
+                for (int j = 0; j < JS; ++j) {
+                    const int r = j * 16 + v_row;
+                    uint32_t b[4];
+                    ldmatrix4_trans(b, vb + r * S::kRowBytes + (((2 * n2 + v_chunk) ^ (r & 7)) << 4));
+#pragma unroll
+                    for (int hg = 0; hg < HG; ++hg) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            mma<KV>(acc[hg][i], pf[hg][j][0][0], pf[hg][j][1][0], pf[hg][j][0][1], pf[hg][j][1][1], b[2 * i], b[2 * i + 1]);
+                            if constexpr (S::kPPlanes > 2) {
+                                mma<KV>(acc[hg][i], pf[hg][j][S::kPPlanes - 1][0], 0u, pf[hg][j][S::kPPlanes - 1][1], 0u, b[2 * i], b[2 * i + 1]);
+                            }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int hg = 0; hg < HG; ++hg)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            o[hg][2 * n2 + i][e] = fmaf(o[hg][2 * n2 + i][e], fade[hg], acc[hg][i][e] + acc[hg][i][2 + e]);
+            }
+            __syncwarp();
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+        }
+
+        // ---- join the warps, 8 heads x 64 dims at a time ----
+        const bool whole_item = seg.t0 == 0 && seg.t1 == seg.tiles;
+        float* part = p.parts + (static_cast<size_t>(blockIdx.x) * 2 + (seg.t0 == 0)) * kSlotFloats;
+#pragma unroll
+        for (int hg = 0; hg < HG; ++hg) {
+            l[hg] += __shfl_xor_sync(0xffffffffu, l[hg], 1);
+            l[hg] += __shfl_xor_sync(0xffffffffu, l[hg], 2);
+#pragma unroll
+            for (int d0 = 0; d0 < HD; d0 += 64) {
+                if (hg + d0 > 0) __syncthreads();  // the values before have been read
+                if (t4 == 0) {
+                    merge_m[warp * 8 + g] = m[hg];
+                    merge_l[warp * 8 + g] = l[hg];
+                }
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    *reinterpret_cast<float2*>(&merge_o[(warp * 8 + g) * 64 + n * 8 + 2 * t4]) = make_float2(o[hg][d0 / 8 + n][0], o[hg][d0 / 8 + n][1]);
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < min(heads - hg * 8, 8) * 64; i += kThreads) {
+                    const int h = i / 64, d = d0 + i % 64;
+                    float mm = -INFINITY, ll = 0.f, v = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, merge_m[w * 8 + h]);
+                    const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float f = exp2f(merge_m[w * 8 + h] - ref);
+                        ll = fmaf(f, merge_l[w * 8 + h], ll);
+                        v = fmaf(f, merge_o[(w * 8 + h) * 64 + i % 64], v);
+                    }
+                    const int row = hg * 8 + h;
+                    if (whole_item) {
+                        if (d < hd) static_cast<X*>(p.out)[(row0 + row) * hd + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
+                        if (d == 0 && p.lse != nullptr) p.lse[row0 + row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
+                    } else {
+                        part[32 + row * HD + d] = v;
+                        if (d == 0) {
+                            part[row] = mm;
+                            part[16 + row] = ll;
+                        }
+                    }
+                }
+            }
+        }
+        if (!whole_item) {
+            // The item's CTAs are those of its flat tiles; the first one's counter tells who comes last.
+            const int c0 = static_cast<int>(seg.at / share), c1 = static_cast<int>((seg.at + seg.tiles - 1) / share);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                __threadfence();
+                const unsigned n = atom_acq_rel_gpu_add(p.arrived + c0, 1u);
+                const bool last = n == static_cast<unsigned>(c1 - c0);
+                if (last) p.arrived[c0] = 0u;
+                shared_word[15] = last;
+                __threadfence();
+            }
+            __syncthreads();
+            if (shared_word[15]) {
+                for (int i = threadIdx.x; i < heads * HD; i += kThreads) {
+                    const int h = i / HD, d = i % HD;
+                    float mm = -INFINITY, ll = 0.f, v = 0.f;
+                    for (int c = c0; c <= c1; ++c) {
+                        const float* q = p.parts + (static_cast<size_t>(c) * 2 + (c == c0)) * kSlotFloats;
+                        mm = fmaxf(mm, __ldcg(q + h));
+                    }
+                    const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll 4
+                    for (int c = c0; c <= c1; ++c) {
+                        const float* q = p.parts + (static_cast<size_t>(c) * 2 + (c == c0)) * kSlotFloats;
+                        const float f = exp2f(__ldcg(q + h) - ref);
+                        ll = fmaf(f, __ldcg(q + 16 + h), ll);
+                        v = fmaf(f, __ldcg(q + 32 + i), v);
+                    }
+                    if (d < hd) static_cast<X*>(p.out)[(row0 + h) * hd + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
+                    if (d == 0 && p.lse != nullptr) p.lse[row0 + h] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
+                }
+            }
+        }
+        if (!next_segment<TILE>(p, walk, seg)) break;
+        __syncthreads();  // the joined values have been read
+    }
+    copy_wait<0>();
+}
+
+template <typename X, typename KV, int HD, int HG>
+void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStream_t stream) {
+    using S = Shape<X, KV, HD, HG>;
+    Params p;
+    p.q = a.q;
+    p.k = static_cast<const char*>(pg.k) + 2 * a.layer * pg.layer_stride;
+    p.v = static_cast<const char*>(pg.v) + 2 * a.layer * pg.layer_stride;
+    p.parts = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kPagedCounterBytes);
+    p.arrived = static_cast<unsigned*>(a.workspace);
+    p.q_seq_stride = a.q_seq_stride;
+    p.q_head_stride = a.q_head_stride;
+    p.table_stride = a.table_stride;
+    p.page_stride = pg.page_stride;
+    p.head_stride = pg.head_stride;
+    p.token_stride = pg.token_stride;
+    p.scale2 = a.scale * kLog2e;
+    p.n_heads = a.n_heads;
+    p.n_pages = pg.n_pages;
+    p.page_size = pg.page_size;
+    p.table_width = a.table_width;
+    p.head_dim = pg.head_dim;
+    p.window = a.window;
+    p.group = a.n_heads / pg.n_kv_heads;
+    p.per_head = (p.group + S::kHeads - 1) / S::kHeads;
+    p.items = p.per_head * pg.n_kv_heads;
+    p.page_div = fast_div(pg.page_size);
+    auto kernel = attend_kernel<X, KV, HD, HG>;
+    static std::atomic<uint64_t> allowed{0};  // devices on which this kernel may use its shared memory
+    int dev = 0;
+    CLLM_CUDA(cudaGetDevice(&dev));
+    if (dev >= 64 || !(allowed.load() >> dev & 1)) {
+        CLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kFixed + 4 * (kMaxRows + 1)));
+        if (dev < 64) allowed.fetch_or(1ull << dev);
+    }
+    const long long cap = static_cast<long long>(a.table_width) * pg.page_size;
+    const long long row_tiles = std::max(1LL, (cap + S::kTile - 1) / S::kTile * p.items);  // most tiles of a sequence
+    CLLM_REQUIRE(row_tiles <= (1LL << 31), "cudallm_paged_attend: the tables are too wide");
+    const int at_once = static_cast<int>(std::min<long long>(kMaxRows, std::max(1LL, (1LL << 31) / row_tiles)));
+    for (int b0 = 0; b0 < a.n_seq; b0 += at_once) {
+        p.n_seq = std::min(at_once, a.n_seq - b0);
+        p.lens = a.lens + b0;
+        p.tables = a.tables + b0 * a.table_stride;
+        p.q = static_cast<const X*>(a.q) + b0 * a.q_seq_stride;
+        p.out = static_cast<X*>(a.out) + static_cast<long long>(b0) * a.n_heads * pg.head_dim;
+        p.lse = a.lse != nullptr ? a.lse + static_cast<long long>(b0) * a.n_heads : nullptr;
+        const size_t smem = S::kFixed + 4 * (static_cast<size_t>(p.n_seq) + 1);
+        const int per_sm = smem <= 113 * 1024 ? 2 : 1;
+        const long long most = std::max<long long>(1, (row_tiles + kWarps - 1) / kWarps * p.n_seq + p.items * static_cast<long long>(p.n_seq));
+        const int grid = static_cast<int>(std::min<long long>(std::min(kMaxCtas, num_sms() * per_sm), most));
+        kernel<<<grid, kThreads, smem, stream>>>(p);
+        CLLM_CUDA(cudaGetLastError());
+    }
+}
+
+template <typename X, typename KV>
+void launch_types(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStream_t stream) {
+    const bool two = a.n_heads / pg.n_kv_heads > 8;  // both groups of 8 heads share one read of the keys
+    if (pg.head_dim <= 64) {
+        two ? launch_shape<X, KV, 64, 2>(pg, a, stream) : launch_shape<X, KV, 64, 1>(pg, a, stream);
+    } else if (pg.head_dim <= 128) {
+        two ? launch_shape<X, KV, 128, 2>(pg, a, stream) : launch_shape<X, KV, 128, 1>(pg, a, stream);
     } else {
-        attend_kernel<X, __half><<<grid, 32 * kWarps, 0, stream>>>(pg, a);
+        launch_shape<X, KV, 256, 1>(pg, a, stream);  // a second group would not fit the registers
     }
 }
 
 }  // namespace
 
-size_t attend_workspace_bytes() { return kPagedCounterBytes; }
+size_t attend_workspace_bytes() { return kPagedCounterBytes + sizeof(float) * kSlotFloats * 2 * kMaxCtas; }
 
 void launch_paged_attend(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStream_t stream) {
     if (a.n_seq == 0) return;
+    const bool bf16 = pg.kv_dtype == CUDALLM_KV_BF16;
     switch (a.x_dtype) {
-        case CUDALLM_X_FP32: launch_for<float>(pg, a, stream); break;
-        case CUDALLM_X_FP16: launch_for<__half>(pg, a, stream); break;
-        default: launch_for<__nv_bfloat16>(pg, a, stream); break;
+        case CUDALLM_X_FP32: bf16 ? launch_types<float, __nv_bfloat16>(pg, a, stream) : launch_types<float, __half>(pg, a, stream); break;
+        case CUDALLM_X_FP16: bf16 ? launch_types<__half, __nv_bfloat16>(pg, a, stream) : launch_types<__half, __half>(pg, a, stream); break;
+        default: bf16 ? launch_types<__nv_bfloat16, __nv_bfloat16>(pg, a, stream) : launch_types<__nv_bfloat16, __half>(pg, a, stream); break;
     }
-    CLLM_CUDA(cudaGetLastError());
 }
 
 }  // namespace cudallm

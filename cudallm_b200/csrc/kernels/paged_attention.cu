@@ -206,6 +206,92 @@ __device__ __forceinline__ bool next_segment(const Params& p, const Walk& w, Seg
     return true;
 }
 
+// Joins the partials of CTAs c0 .. c1 of an item of `heads` query heads in order, and writes its rows. All of the block's threads; `o` has
+// room for kWarps * 512 floats and `stat` for 64. Every thread owns four dims of a head and one in `ways` of the partials, whose loads
+// are all independent of each other: what the join costs is two or three round trips to L2.
+constexpr int kJoin = 128;  // partials whose weights are held at once
+template <typename X, int HD>
+__device__ __noinline__ void join_parts(const Params& p, int c0, int c1, int heads, long long row0, float* o, float* stat) {
+    float* weight = o;                     // [8 heads][kJoin]
+    float* sums = o + 8 * kJoin;           // [ways][columns][4]: kThreads float4
+    float *top = stat, *total = stat + 8, *fade = stat + 16;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    auto part_of = [&](int c) { return p.parts + (static_cast<size_t>(c) * 2 + (c == c0)) * kSlotFloats; };
+    for (int h0 = 0; h0 < heads; h0 += 8) {
+        const int n_heads = min(heads - h0, 8);
+        for (int d0 = 0; d0 < HD; d0 += 64) {
+            const int columns = n_heads * 16;  // float4s of 64 dims
+            int ways = 1;
+            while (ways * 2 * columns <= kThreads) ways *= 2;
+            const int col = threadIdx.x % columns, way = threadIdx.x / columns;
+            const int h = col / 16, d = d0 + col % 16 * 4;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (threadIdx.x < 8) {
+                top[threadIdx.x] = -INFINITY;
+                total[threadIdx.x] = 0.f;
+            }
+            for (int from = c0; from <= c1; from += kJoin) {
+                const int n = min(c1 + 1 - from, kJoin);
+                __syncthreads();
+                for (int hh = warp; hh < n_heads; hh += kWarps) {
+                    float m[kJoin / 32], l[kJoin / 32], mm = top[hh];
+                    const float before = mm;
+#pragma unroll
+                    for (int k = 0; k < kJoin / 32; ++k) {
+                        const int c = lane + 32 * k;
+                        m[k] = c < n ? __ldcg(part_of(from + c) + h0 + hh) : -INFINITY;
+                        l[k] = c < n ? __ldcg(part_of(from + c) + 16 + h0 + hh) : 0.f;
+                        mm = fmaxf(mm, m[k]);
+                    }
+#pragma unroll
+                    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+                    const float ref = mm == -INFINITY ? 0.f : mm, old = exp2f(before - ref);
+                    float sum = 0.f;
+#pragma unroll
+                    for (int k = 0; k < kJoin / 32; ++k) {
+                        const float w = exp2f(m[k] - ref);
+                        weight[hh * kJoin + lane + 32 * k] = w;
+                        sum = fmaf(w, l[k], sum);
+                    }
+#pragma unroll
+                    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+                    __syncwarp();
+                    if (lane == 0) {
+                        total[hh] = fmaf(total[hh], old, sum);
+                        top[hh] = mm;
+                        fade[hh] = old;
+                    }
+                }
+                __syncthreads();
+                if (way < ways) {
+                    const float f = fade[h];
+                    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
+#pragma unroll 8
+                    for (int c = way; c < n; c += ways) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(from + c) + 32 + (h0 + h) * HD + d));
+                        const float w = weight[h * kJoin + c];
+                        acc.x = fmaf(w, v.x, acc.x);
+                        acc.y = fmaf(w, v.y, acc.y);
+                        acc.z = fmaf(w, v.z, acc.z);
+                        acc.w = fmaf(w, v.w, acc.w);
+                    }
+                }
+            }
+            if (way < ways) reinterpret_cast<float4*>(sums)[way * columns + col] = acc;
+            __syncthreads();
+            for (int i = threadIdx.x; i < n_heads * 64; i += kThreads) {
+                const int hh = i / 64, dim = d0 + i % 64;
+                float v = 0.f;
+                for (int w = 0; w < ways; ++w) v += sums[(w * columns) * 4 + i];
+                const float l = total[hh];
+                if (dim < p.head_dim) static_cast<X*>(p.out)[(row0 + h0 + hh) * p.head_dim + dim] = from_float<X>(l > 0.f ? v / l : 0.f);
+                if (dim == 0 && p.lse != nullptr) p.lse[row0 + h0 + hh] = l > 0.f ? fmaf(top[hh], kLn2, logf(l)) : -INFINITY;
+            }
+            __syncthreads();
+        }
+    }
+}
+
 template <typename X, typename KV, int HD, int HG>
 __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ Params p) {
     using S = Shape<X, KV, HD, HG>;
@@ -588,26 +674,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
                 __threadfence();
             }
             __syncthreads();
-            if (shared_word[15]) {
-                for (int i = threadIdx.x; i < heads * HD; i += kThreads) {
-                    const int h = i / HD, d = i % HD;
-                    float mm = -INFINITY, ll = 0.f, v = 0.f;
-                    for (int c = c0; c <= c1; ++c) {
-                        const float* q = p.parts + (static_cast<size_t>(c) * 2 + (c == c0)) * kSlotFloats;
-                        mm = fmaxf(mm, __ldcg(q + h));
-                    }
-                    const float ref = mm == -INFINITY ? 0.f : mm;
-#pragma unroll 4
-                    for (int c = c0; c <= c1; ++c) {
-                        const float* q = p.parts + (static_cast<size_t>(c) * 2 + (c == c0)) * kSlotFloats;
-                        const float f = exp2f(__ldcg(q + h) - ref);
-                        ll = fmaf(f, __ldcg(q + 16 + h), ll);
-                        v = fmaf(f, __ldcg(q + 32 + i), v);
-                    }
-                    if (d < hd) static_cast<X*>(p.out)[(row0 + h) * hd + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
-                    if (d == 0 && p.lse != nullptr) p.lse[row0 + h] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
-                }
-            }
+            if (shared_word[15]) join_parts<X, HD>(p, c0, c1, heads, row0, merge_o, merge_m);
         }
         if (!next_segment<TILE>(p, walk, seg)) break;
         __syncthreads();  // the joined values have been read

@@ -9,11 +9,11 @@
 // Split. The positions of all (sequence, key head) items are cut into tiles of kTile tokens and counted through from
 // first to last; CTA c takes tiles [c Q, (c + 1) Q), so ragged lengths spread evenly and one long sequence covers the
 // GPU. A CTA's part of an item is a segment; the warps of the CTA take its tiles in turn, each with its own running (m,
-// sum, out), which are joined in warp order. Segments that are not a whole item are left in the workspace, and the
-// last CTA of the item to arrive joins them in order: no result depends on the order of arrival.
+// sum, out), which are joined in warp order. Segments that are not a whole item are left in the workspace, and a second
+// kernel, whose blocks are already in place when the last of them is written, joins them in the order of the CTAs.
 //
 // Tiles. A warp copies its tiles with 16-byte asynchronous copies into a ring of its own (no block barrier between
-// tiles), three deep; each lane looks up the page of one token, so pages of any size may end inside a tile. Rows are
+// tiles), two or three deep; each lane looks up the page of one token, so pages of any size may end inside a tile. Rows are
 // swizzled (chunk ^ row % 8) so that ldmatrix reads them without bank conflicts. Tokens without a page, outside the
 // window or past the length are filled with zeros instead of being read, and masked by one bit each.
 //
@@ -27,9 +27,11 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 #include "common/check.h"
 #include "kernels/kernels.h"
+#include "kernels/launch.cuh"
 #include "kernels/paged.h"
 #include "kernels/paged_common.cuh"
 #include "kernels/ptx.cuh"
@@ -40,11 +42,13 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kStages = 3;
 constexpr int kMaxCtas = 512;
 constexpr int kMaxRows = 2048;          // sequences of one launch (their tile counts are summed in shared memory)
 constexpr int kSlotFloats = 16 * 2 + 16 * 128;  // a partial: m, sum and out of 16 heads x 128 dims or 8 x 256
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+constexpr size_t kEndingBytes = 32 * kMaxCtas;
+constexpr int kUnit = 8;  // tiles of a CTA where there are few
 
 // n / d for 0 <= n < 2^31 as a multiplication.
 struct FastDiv {
@@ -59,6 +63,12 @@ __device__ __forceinline__ int div_by(int n, FastDiv f) {
     return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(n)) * f.mul) >> f.shift);
 }
 
+// What a CTA's first segment is the last part of: the partials of CTAs c0 .. c0 + n - 1 make up `heads` rows of the output (n = 0: nothing).
+struct __align__(16) Ending {
+    int n, c0, heads, pad;
+    long long row0;
+};
+
 struct Params {
     const void* q;
     const char* k;  // the layer's pages
@@ -67,8 +77,8 @@ struct Params {
     float* lse;
     const int* tables;
     const int* lens;
-    float* parts;       // [CTA][2] partials
-    unsigned* arrived;  // [CTA]
+    float* parts;  // [CTA][2] partials
+    Ending* endings;  // [CTA]
     long long q_seq_stride, q_head_stride, table_stride, page_stride, head_stride, token_stride;  // elements
     float scale2;                                                                                  // scale * log2(e)
     int n_seq, n_heads, n_pages, page_size, table_width, head_dim, window;
@@ -76,6 +86,9 @@ struct Params {
     int per_head;   // items per key head (groups of 8 HG query heads)
     int items;      // items per sequence
     FastDiv page_div;
+    bool long_runs;      // page_size % 16 == 0: 16 tokens from a multiple of 16 on lie in one page
+    bool dense;          // a head's tokens are HD dims apart and have as many
+    long long row_step;  // bytes between the rows of one copy instruction and the next
 };
 
 template <typename KV>
@@ -92,6 +105,20 @@ __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, u
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same product with nothing to add to.
+template <typename KV>
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<KV, __nv_bfloat16>) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    }
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -120,45 +147,54 @@ __device__ __forceinline__ void copy_wait() {
 // (a, b) rounded to the cache's type and packed, a in the low half; a and b keep what the rounding left.
 template <typename KV>
 __device__ __forceinline__ uint32_t take_plane(float& a, float& b) {
-    const KV ha = from_float<KV>(a), hb = from_float<KV>(b);
-    a -= as_float(ha);
-    b -= as_float(hb);
-    uint16_t ua, ub;
-    memcpy(&ua, &ha, 2);
-    memcpy(&ub, &hb, 2);
-    return static_cast<uint32_t>(ub) << 16 | ua;
+    uint32_t bits;
+    if constexpr (std::is_same_v<KV, __nv_bfloat16>) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        memcpy(&bits, &h, 4);
+        a -= __uint_as_float(bits << 16);
+        b -= __uint_as_float(bits & 0xffff0000u);
+    } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        memcpy(&bits, &h, 4);
+        a -= __low2float(h);
+        b -= __high2float(h);
+    }
+    return bits;
 }
 
-template <typename A, typename B>
-struct Same {
-    static constexpr bool value = false;
-};
-template <typename A>
-struct Same<A, A> {
-    static constexpr bool value = true;
-};
+// 2^x to 22 bits; results below the normal range are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // HD: head dims rounded up to 64, 128 or 256; HG: groups of 8 query heads of an item.
 template <typename X, typename KV, int HD, int HG>
 struct Shape {
-    static constexpr bool kBf16 = Same<KV, __nv_bfloat16>::value, kF32 = Same<X, float>::value;
-    static constexpr int kQPlanes = Same<X, KV>::value ? 1 : kBf16 && kF32 ? 3 : 2;
+    static constexpr bool kBf16 = std::is_same_v<KV, __nv_bfloat16>, kF32 = std::is_same_v<X, float>;
+    static constexpr int kQPlanes = std::is_same_v<X, KV> ? 1 : kBf16 && kF32 ? 3 : 2;
     static constexpr int kPPlanes = kBf16 && kF32 ? 3 : 2;
+    static constexpr bool kScaleQ = !kBf16 && kQPlanes > 1;
     static constexpr int kTile = HD == 64 ? 32 : 16;  // tokens
+    static constexpr int kStages = HD == 256 || HG == 2 ? 3 : 2;
+    static constexpr int kCtas = HD == 256 ? 1 : HG == 2 ? 2 : 3;  // resident on an SM, by shared memory and registers
     static constexpr int kRowBytes = HD * 2;
     static constexpr int kPlaneBytes = kTile * kRowBytes;  // keys or values of a tile
     static constexpr int kStageBytes = 2 * kPlaneBytes;
     static constexpr int kHeads = 8 * HG;
     static constexpr int kRing = kWarps * kStages * kStageBytes;
-    static constexpr int kMerge = kWarps * 8 * (64 + 2) * 4;  // the warps' results of 8 heads x 64 dims
-    static constexpr int kFixed = kRing + kMerge + kWarps * kStages * 4 + 64;
+    static constexpr int kQWords = HG * (HD / 16) * kQPlanes * 2 * 32;  // an item's query as matrix operands
+    static constexpr int kJoin = (kWarps - 1) * (8 * 64 + 16) * 4;      // all but one warp's out, m and sum of 8 heads x 64 dims
+    static constexpr int kFixed = kRing + kJoin + kQWords * 4 + kWarps * (kStages + 8 * HG) * 4 + 64;
 };
 
 struct Segment {
-    int b, item;       // sequence, item of it
+    int b, item;        // sequence, item of it
     int t0, t1, tiles;  // [t0, t1) of the item's tiles
-    unsigned at;       // flat number of the item's first tile
-    int first_tile;    // of the sequence: where the window starts
+    unsigned at;        // flat number of the item's first tile
+    int len, first;     // the sequence's positions are [first, len)
+    int first_tile;     // the tile of `first`
 };
 
 // One CTA's walk over its flat range of tiles.
@@ -180,10 +216,9 @@ __device__ __forceinline__ void tiles_of(const Params& p, int b, int& len, int& 
 // The segment of sequence b, item `item` from flat tile f on.
 template <int TILE>
 __device__ __forceinline__ void open_segment(const Params& p, const Walk& w, Segment& s, int b, int item, unsigned f) {
-    int len, first;
     s.b = b;
     s.item = item;
-    tiles_of<TILE>(p, b, len, first, s.first_tile, s.tiles);
+    tiles_of<TILE>(p, b, s.len, s.first, s.first_tile, s.tiles);
     const unsigned padded = w.before[b + 1] - w.before[b];
     s.at = w.before[b] * w.items + item * padded;
     s.t0 = static_cast<int>(f - s.at);
@@ -206,108 +241,27 @@ __device__ __forceinline__ bool next_segment(const Params& p, const Walk& w, Seg
     return true;
 }
 
-// Joins the partials of CTAs c0 .. c1 of an item of `heads` query heads in order, and writes its rows. All of the block's threads; `o` has
-// room for kWarps * 512 floats and `stat` for 64. Every thread owns four dims of a head and one in `ways` of the partials, whose loads
-// are all independent of each other: what the join costs is two or three round trips to L2.
-constexpr int kJoin = 128;  // partials whose weights are held at once
-template <typename X, int HD>
-__device__ __noinline__ void join_parts(const Params& p, int c0, int c1, int heads, long long row0, float* o, float* stat) {
-    float* weight = o;                     // [8 heads][kJoin]
-    float* sums = o + 8 * kJoin;           // [ways][columns][4]: kThreads float4
-    float *top = stat, *total = stat + 8, *fade = stat + 16;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    auto part_of = [&](int c) { return p.parts + (static_cast<size_t>(c) * 2 + (c == c0)) * kSlotFloats; };
-    for (int h0 = 0; h0 < heads; h0 += 8) {
-        const int n_heads = min(heads - h0, 8);
-        for (int d0 = 0; d0 < HD; d0 += 64) {
-            const int columns = n_heads * 16;  // float4s of 64 dims
-            int ways = 1;
-            while (ways * 2 * columns <= kThreads) ways *= 2;
-            const int col = threadIdx.x % columns, way = threadIdx.x / columns;
-            const int h = col / 16, d = d0 + col % 16 * 4;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (threadIdx.x < 8) {
-                top[threadIdx.x] = -INFINITY;
-                total[threadIdx.x] = 0.f;
-            }
-            for (int from = c0; from <= c1; from += kJoin) {
-                const int n = min(c1 + 1 - from, kJoin);
-                __syncthreads();
-                for (int hh = warp; hh < n_heads; hh += kWarps) {
-                    float m[kJoin / 32], l[kJoin / 32], mm = top[hh];
-                    const float before = mm;
-#pragma unroll
-                    for (int k = 0; k < kJoin / 32; ++k) {
-                        const int c = lane + 32 * k;
-                        m[k] = c < n ? __ldcg(part_of(from + c) + h0 + hh) : -INFINITY;
-                        l[k] = c < n ? __ldcg(part_of(from + c) + 16 + h0 + hh) : 0.f;
-                        mm = fmaxf(mm, m[k]);
-                    }
-#pragma unroll
-                    for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
-                    const float ref = mm == -INFINITY ? 0.f : mm, old = exp2f(before - ref);
-                    float sum = 0.f;
-#pragma unroll
-                    for (int k = 0; k < kJoin / 32; ++k) {
-                        const float w = exp2f(m[k] - ref);
-                        weight[hh * kJoin + lane + 32 * k] = w;
-                        sum = fmaf(w, l[k], sum);
-                    }
-#pragma unroll
-                    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-                    __syncwarp();
-                    if (lane == 0) {
-                        total[hh] = fmaf(total[hh], old, sum);
-                        top[hh] = mm;
-                        fade[hh] = old;
-                    }
-                }
-                __syncthreads();
-                if (way < ways) {
-                    const float f = fade[h];
-                    acc = make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f);
-#pragma unroll 8
-                    for (int c = way; c < n; c += ways) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_of(from + c) + 32 + (h0 + h) * HD + d));
-                        const float w = weight[h * kJoin + c];
-                        acc.x = fmaf(w, v.x, acc.x);
-                        acc.y = fmaf(w, v.y, acc.y);
-                        acc.z = fmaf(w, v.z, acc.z);
-                        acc.w = fmaf(w, v.w, acc.w);
-                    }
-                }
-            }
-            if (way < ways) reinterpret_cast<float4*>(sums)[way * columns + col] = acc;
-            __syncthreads();
-            for (int i = threadIdx.x; i < n_heads * 64; i += kThreads) {
-                const int hh = i / 64, dim = d0 + i % 64;
-                float v = 0.f;
-                for (int w = 0; w < ways; ++w) v += sums[(w * columns) * 4 + i];
-                const float l = total[hh];
-                if (dim < p.head_dim) static_cast<X*>(p.out)[(row0 + h0 + hh) * p.head_dim + dim] = from_float<X>(l > 0.f ? v / l : 0.f);
-                if (dim == 0 && p.lse != nullptr) p.lse[row0 + h0 + hh] = l > 0.f ? fmaf(top[hh], kLn2, logf(l)) : -INFINITY;
-            }
-            __syncthreads();
-        }
-    }
-}
-
 template <typename X, typename KV, int HD, int HG>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_kernel(const __grid_constant__ Params p) {
     using S = Shape<X, KV, HD, HG>;
+    constexpr int kStages = S::kStages;
     constexpr int TILE = S::kTile, NT = TILE / 8, KS = HD / 16, JS = TILE / 16;
     extern __shared__ __align__(128) char smem[];
     char* ring = smem;
-    float* merge_o = reinterpret_cast<float*>(smem + S::kRing);  // [warp][8 heads][64 dims]
-    float* merge_m = merge_o + kWarps * 8 * 64;                  // [warp][8]
-    float* merge_l = merge_m + kWarps * 8;
-    unsigned* masks = reinterpret_cast<unsigned*>(merge_l + kWarps * 8);  // [warp][stage]
-    unsigned* shared_word = masks + kWarps * kStages;                     // [16]
-    unsigned* before = reinterpret_cast<unsigned*>(smem + S::kFixed);     // [n_seq + 1]
+    float* join_o = reinterpret_cast<float*>(smem + S::kRing);                       // [kWarps - 1][16 floats a lane, 4 at a time]
+    float* join_m = join_o + (kWarps - 1) * 512;                                     // [kWarps - 1][8]
+    float* join_l = join_m + (kWarps - 1) * 8;                                       // [kWarps - 1][8]
+    uint32_t* q_words = reinterpret_cast<uint32_t*>(join_l + (kWarps - 1) * 8);      // [hg][ks][plane][2][lane]
+    unsigned* masks = q_words + S::kQWords;                                          // [warp][stage]
+    float* q_tops = reinterpret_cast<float*>(masks + kWarps * kStages);              // [warp][head]
+    unsigned* shared_word = reinterpret_cast<unsigned*>(q_tops + kWarps * 8 * HG);   // [16]
+    unsigned* before = reinterpret_cast<unsigned*>(smem + S::kFixed);                // [n_seq + 1]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t4 = lane & 3, hd = p.head_dim;
+    if (threadIdx.x == 0) p.endings[blockIdx.x].n = 0;
+    grid_dep_launch();  // the join's blocks may take the places that this kernel's leave
 
-    // Tiles of one item before each sequence, as they are and rounded up to kWarps; empty rows are answered here.
+    // Tiles of one item before each sequence, as they are and in units of kUnit; empty rows are answered here.
     unsigned total = 0, total_pad = 0;
     for (int b0 = 0; b0 < p.n_seq; b0 += kThreads) {
         const int b = b0 + threadIdx.x;
@@ -319,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
             const unsigned t = __shfl_up_sync(0xffffffffu, s, o);
             if (lane >= o) s += t;
         }
-        const unsigned pads = __reduce_add_sync(0xffffffffu, (tiles + kWarps - 1) / kWarps);
+        const unsigned pads = __reduce_add_sync(0xffffffffu, (tiles + kUnit - 1) / kUnit);
         if (lane == 31) {
             shared_word[warp] = s;
             shared_word[kWarps + warp] = pads;
@@ -344,16 +298,16 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
             for (int h = threadIdx.x; h < p.n_heads; h += kThreads) p.lse[static_cast<long long>(b) * p.n_heads + h] = -INFINITY;
         }
     }
-    // Few tiles: an item's tiles are cut every kWarps, one tile a warp. Otherwise every CTA takes an equal share.
+    // Few tiles: an item's tiles are cut every kUnit. Otherwise every CTA takes an equal share.
     const bool few = total_pad * p.items <= gridDim.x;
-    const unsigned share = few ? kWarps : (total * p.items + gridDim.x - 1) / gridDim.x;
-    const unsigned all = few ? total_pad * kWarps * p.items : total * p.items;
+    const unsigned share = few ? kUnit : (total * p.items + gridDim.x - 1) / gridDim.x;
+    const unsigned all = few ? total_pad * kUnit * p.items : total * p.items;
     __syncthreads();
     if (few) {  // the same sums of rounded tile counts
         unsigned run = 0;
         for (int b0 = 0; b0 < p.n_seq; b0 += kThreads) {
             const int b = b0 + threadIdx.x;
-            const unsigned mine = b < p.n_seq ? (before[b + 1] - before[b] + kWarps - 1) / kWarps * kWarps : 0;
+            const unsigned mine = b < p.n_seq ? (before[b + 1] - before[b] + kUnit - 1) / kUnit * kUnit : 0;
             unsigned s = mine;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -374,7 +328,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
         __syncthreads();
     }
     const unsigned f0 = min(all, blockIdx.x * share);
-    Walk walk{before, p.n_seq, p.items, few ? kWarps : 1, min(all, f0 + share)};
+    Walk walk{before, p.n_seq, p.items, few ? kUnit : 1, min(all, f0 + share)};
     if (f0 >= walk.f1) return;
 
     // The first segment: the last sequence that starts at or before f0.
@@ -390,6 +344,73 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
         open_segment<TILE>(p, walk, seg, lo, static_cast<int>((f0 - before[lo] * p.items) / padded), f0);
     }
 
+    // ---- the query, as operands in shared memory: warp w turns k-steps w, w + kWarps, ... of the next segment ----
+    constexpr int QS = (KS + kWarps - 1) / kWarps;
+    float raw[HG][QS][4];
+    auto fetch_q = [&](const Segment& s) {
+        const int kvh = s.item / p.per_head, h_first = (s.item % p.per_head) * S::kHeads;
+#pragma unroll
+        for (int hg = 0; hg < HG; ++hg) {
+            const int h = h_first + hg * 8 + g;
+            const X* q = static_cast<const X*>(p.q) + s.b * p.q_seq_stride + (kvh * p.group + h) * p.q_head_stride;
+#pragma unroll
+            for (int i = 0; i < QS; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = (i * kWarps + warp) * 16 + 2 * t4 + (e & 1) + (e >> 1) * 8;
+                    raw[hg][i][e] = h < p.group && d < hd ? as_float(q[d]) : 0.f;
+                }
+            }
+        }
+    };
+    auto put_tops = [&] {  // largest |q| of this warp's dims
+        if constexpr (S::kScaleQ) {
+#pragma unroll
+            for (int hg = 0; hg < HG; ++hg) {
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < QS; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(raw[hg][i][e]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                if (t4 == 0) q_tops[warp * 8 * HG + hg * 8 + g] = top;
+            }
+        }
+    };
+    float q_scale[HG];
+    auto put_q = [&] {  // after a barrier behind put_tops
+#pragma unroll
+        for (int hg = 0; hg < HG; ++hg) {
+            float shrink = 1.f;
+            q_scale[hg] = p.scale2;
+            if constexpr (S::kScaleQ) {
+                // fp16 planes: the head is brought to 1 <= max|q| < 2 by a power of two, which the scale gives back.
+                float top = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, q_tops[w * 8 * HG + hg * 8 + g]);
+                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253) - 127;
+                shrink = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+                q_scale[hg] *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+            }
+#pragma unroll
+            for (int i = 0; i < QS; ++i) {
+                const int ks = i * kWarps + warp;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = raw[hg][i][e] * shrink;
+#pragma unroll
+                for (int pl = 0; pl < S::kQPlanes; ++pl) {
+                    uint32_t* w = q_words + ((hg * KS + ks) * S::kQPlanes + pl) * 64 + lane;
+                    w[0] = take_plane<KV>(v[0], v[1]);
+                    w[32] = take_plane<KV>(v[2], v[3]);
+                }
+            }
+        }
+    };
+    static_assert(KS % kWarps == 0, "every warp turns as many k-steps");
+    fetch_q(seg);  // on its way while the first tiles are looked up
+
     // ---- the warp's stream of tiles ----
     Segment ls = seg;                  // of the next tile to load
     int lt = ls.t0 + warp;             // that tile
@@ -398,16 +419,19 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
     int l_page = -1;
     bool l_valid = false;
     const uint32_t my_ring = smem_addr(ring) + warp * (kStages * S::kStageBytes);
+    // One copy instruction of the warp covers kRowsAtOnce rows; this lane takes 16-byte chunk lane % kChunks of row lane / kChunks.
+    constexpr int kChunks = HD / 8, kRowsAtOnce = 32 / kChunks;
+    const int inside = lane % kChunks * 8 < hd ? 16 : 0;
+    const uint32_t my_dst = lane / kChunks * S::kRowBytes + ((lane % kChunks ^ lane / kChunks) << 4);
+    const long long my_src = inside ? lane / kChunks * p.token_stride * 2 + lane % kChunks * 16 : 0;
     auto look_up = [&] {  // moves to the next tile of this warp and reads its lane's page number
         while (more && lt >= ls.t1) {
             more = next_segment<TILE>(p, walk, ls);
             lt = ls.t0 + warp;
         }
         if (!more) return;
-        int len, first, ft, tiles;
-        tiles_of<TILE>(p, ls.b, len, first, ft, tiles);
         l_token = (ls.first_tile + lt) * TILE + (lane % TILE);
-        l_valid = l_token >= first && l_token < len;
+        l_valid = l_token >= ls.first && l_token < ls.len;
         const int entry = div_by(l_token, p.page_div);
         l_slot = l_token - entry * p.page_size;
         l_page = l_valid ? p.tables[ls.b * p.table_stride + entry] : -1;
@@ -418,19 +442,36 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
             const long long off = valid ? (l_page * p.page_stride + l_slot * p.token_stride + ls.item / p.per_head * p.head_stride) * 2 : -1;
             const unsigned mask = __ballot_sync(0xffffffffu, valid);
             if (lane == 0) masks[warp * kStages + stage] = mask;
-            constexpr int kChunks = HD / 8, kRowsAtOnce = 32 / (kChunks < 32 ? kChunks : 32);
-            const int c = lane % kChunks;
-            const bool inside = c * 8 < hd;
-            const uint32_t dst = my_ring + stage * S::kStageBytes;
+            const uint32_t dst = my_ring + stage * S::kStageBytes + my_dst;
+            if (mask == 0xffffffffu && p.long_runs) {  // 16 tokens at a time lie in one page, evenly spaced
 #pragma unroll
-            for (int r0 = 0; r0 < TILE; r0 += kRowsAtOnce) {
-                const int r = r0 + lane / kChunks;
-                const long long o = __shfl_sync(0xffffffffu, off, r);
-                const int bytes = o >= 0 && inside ? 16 : 0;
-                const long long at = bytes ? o + c * 16 : 0;
-                const uint32_t d = dst + r * S::kRowBytes + ((c ^ (r & 7)) << 4);
-                copy16(d, p.k + at, bytes);
-                copy16(d + S::kPlaneBytes, p.v + at, bytes);
+                for (int r16 = 0; r16 < TILE; r16 += 16) {
+                    const long long o = __shfl_sync(0xffffffffu, off, r16) + my_src;
+                    const char *k = p.k + o, *v = p.v + o;
+#pragma unroll
+                    for (int r0 = r16; r0 < r16 + 16; r0 += kRowsAtOnce) {
+                        const uint32_t d = (dst ^ ((r0 & 7) << 4)) + r0 * S::kRowBytes;
+                        if (p.dense) {
+                            copy16(d, k + (r0 - r16) * S::kRowBytes, 16);
+                            copy16(d + S::kPlaneBytes, v + (r0 - r16) * S::kRowBytes, 16);
+                        } else {
+                            copy16(d, k, inside);
+                            copy16(d + S::kPlaneBytes, v, inside);
+                            k += p.row_step;
+                            v += p.row_step;
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r0 = 0; r0 < TILE; r0 += kRowsAtOnce) {
+                    const long long o = __shfl_sync(0xffffffffu, off, r0 + lane / kChunks);
+                    const int bytes = o >= 0 ? inside : 0;
+                    const long long at = bytes ? o + lane % kChunks * 16 : 0;
+                    const uint32_t d = (dst ^ ((r0 & 7) << 4)) + r0 * S::kRowBytes;
+                    copy16(d, p.k + at, bytes);
+                    copy16(d + S::kPlaneBytes, p.v + at, bytes);
+                }
             }
             lt += kWarps;
         }
@@ -443,7 +484,12 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
         look_up();
     }
 
-    int stage = 0;
+    put_tops();
+    __syncthreads();
+    put_q();
+    __syncthreads();
+
+    int stage = 0, joiner = 0;
     for (;;) {
         // ---- one segment ----
         const int kvh = seg.item / p.per_head, h_first = (seg.item % p.per_head) * S::kHeads;
@@ -451,44 +497,11 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
         const long long row0 = static_cast<long long>(seg.b) * p.n_heads + kvh * p.group + h_first;
 
         uint32_t qf[HG][KS][S::kQPlanes][2];  // planes of q: dims 16 ks + 2 t4 + {0, 1} and + 8
-        float q_scale[HG];
 #pragma unroll
-        for (int hg = 0; hg < HG; ++hg) {
-            const int h = hg * 8 + g;
-            const X* q = static_cast<const X*>(p.q) + seg.b * p.q_seq_stride + (kvh * p.group + h_first + h) * p.q_head_stride;
-            float raw[KS][4];
-            float top = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int d = ks * 16 + 2 * t4 + (e & 1) + (e >> 1) * 8;
-                    raw[ks][e] = h < heads && d < hd ? as_float(q[d]) : 0.f;
-                    top = fmaxf(top, fabsf(raw[ks][e]));
-                }
-            }
-            q_scale[hg] = p.scale2;
-            float shrink = 1.f;
-            if constexpr (!S::kBf16 && S::kQPlanes > 1) {
-                // fp16 planes: the head is brought to 1 <= max|q| < 2 by a power of two, which the scale gives back.
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253) - 127;
-                shrink = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-                q_scale[hg] *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                float v[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = raw[ks][e] * shrink;
-#pragma unroll
-                for (int pl = 0; pl < S::kQPlanes; ++pl) {
-                    qf[hg][ks][pl][0] = take_plane<KV>(v[0], v[1]);
-                    qf[hg][ks][pl][1] = take_plane<KV>(v[2], v[3]);
-                }
-            }
-        }
+        for (int i = 0; i < HG * KS * S::kQPlanes * 2; ++i) (&qf[0][0][0][0])[i] = q_words[i * 32 + lane];
+        Segment following = seg;
+        const bool goes_on = next_segment<TILE>(p, walk, following);
+        if (goes_on) fetch_q(following);
 
         float o[HG][HD / 8][2], m[HG], l[HG];
 #pragma unroll
@@ -509,12 +522,6 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 
             // scores
             float s[HG][NT][4];
-#pragma unroll
-            for (int hg = 0; hg < HG; ++hg)
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[hg][n][e] = 0.f;
             const int k_row = (lane >> 4) * 8 + (lane & 7), k_chunk = (lane >> 3) & 1;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -528,8 +535,12 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
                     for (int hg = 0; hg < HG; ++hg) {
                         const uint32_t lo0 = S::kQPlanes > 1 ? qf[hg][ks][S::kQPlanes > 1][0] : 0u;
                         const uint32_t lo1 = S::kQPlanes > 1 ? qf[hg][ks][S::kQPlanes > 1][1] : 0u;
-                        mma<KV>(s[hg][2 * n2], qf[hg][ks][0][0], lo0, qf[hg][ks][0][1], lo1, b[0], b[1]);
-                        mma<KV>(s[hg][2 * n2 + 1], qf[hg][ks][0][0], lo0, qf[hg][ks][0][1], lo1, b[2], b[3]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float(&c)[4] = s[hg][2 * n2 + i];
+                            if (ks == 0) mma_first<KV>(c, qf[hg][ks][0][0], lo0, qf[hg][ks][0][1], lo1, b[2 * i], b[2 * i + 1]);
+                            else mma<KV>(c, qf[hg][ks][0][0], lo0, qf[hg][ks][0][1], lo1, b[2 * i], b[2 * i + 1]);
+                        }
                         if constexpr (S::kQPlanes > 2) {
                             mma<KV>(s[hg][2 * n2], qf[hg][ks][2][0], 0u, qf[hg][ks][2][1], 0u, b[0], b[1]);
                             mma<KV>(s[hg][2 * n2 + 1], qf[hg][ks][2][0], 0u, qf[hg][ks][2][1], 0u, b[2], b[3]);
@@ -558,14 +569,14 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 const float m_new = fmaxf(m[hg], top), ref = m_new == -INFINITY ? 0.f : m_new;
-                fade[hg] = exp2f(m[hg] - ref);
+                fade[hg] = exp2_fast(m[hg] - ref);
                 m[hg] = m_new;
                 float sum = 0.f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        x[n][e] = exp2f(x[n][e] - ref);
+                        x[n][e] = exp2_fast(x[n][e] - ref);
                         sum += x[n][e];
                     }
                 }
@@ -583,12 +594,6 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
                 if (n2 * 16 >= hd) break;
                 float acc[HG][2][4];
 #pragma unroll
-                for (int hg = 0; hg < HG; ++hg)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[hg][i][e] = 0.f;
-#pragma unroll
                 for (int j = 0; j < JS; ++j) {
                     const int r = j * 16 + v_row;
                     uint32_t b[4];
@@ -597,7 +602,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
                     for (int hg = 0; hg < HG; ++hg) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            mma<KV>(acc[hg][i], pf[hg][j][0][0], pf[hg][j][1][0], pf[hg][j][0][1], pf[hg][j][1][1], b[2 * i], b[2 * i + 1]);
+                            if (j == 0) mma_first<KV>(acc[hg][i], pf[hg][j][0][0], pf[hg][j][1][0], pf[hg][j][0][1], pf[hg][j][1][1], b[2 * i], b[2 * i + 1]);
+                            else mma<KV>(acc[hg][i], pf[hg][j][0][0], pf[hg][j][1][0], pf[hg][j][0][1], pf[hg][j][1][1], b[2 * i], b[2 * i + 1]);
                             if constexpr (S::kPPlanes > 2) {
                                 mma<KV>(acc[hg][i], pf[hg][j][S::kPPlanes - 1][0], 0u, pf[hg][j][S::kPPlanes - 1][1], 0u, b[2 * i], b[2 * i + 1]);
                             }
@@ -616,70 +622,164 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
             stage = stage + 1 == kStages ? 0 : stage + 1;
         }
 
-        // ---- join the warps, 8 heads x 64 dims at a time ----
+        // ---- join the warps: one of them, in turn, adds the others' 8 heads x 64 dims to its own ----
         const bool whole_item = seg.t0 == 0 && seg.t1 == seg.tiles;
         float* part = p.parts + (static_cast<size_t>(blockIdx.x) * 2 + (seg.t0 == 0)) * kSlotFloats;
+        const int others = (warp - joiner - 1) & (kWarps - 1);  // place of this warp's values; the joiner has none
+        if (goes_on) put_tops();
 #pragma unroll
         for (int hg = 0; hg < HG; ++hg) {
             l[hg] += __shfl_xor_sync(0xffffffffu, l[hg], 1);
             l[hg] += __shfl_xor_sync(0xffffffffu, l[hg], 2);
 #pragma unroll
             for (int d0 = 0; d0 < HD; d0 += 64) {
-                if (hg + d0 > 0) __syncthreads();  // the values before have been read
-                if (t4 == 0) {
-                    merge_m[warp * 8 + g] = m[hg];
-                    merge_l[warp * 8 + g] = l[hg];
-                }
+                __syncthreads();  // the values before have been read, and every warp has this segment's query
+                if (hg + d0 == 0 && goes_on) put_q();
+                if (warp != joiner) {
+                    if (t4 == 0) {
+                        join_m[others * 8 + g] = m[hg];
+                        join_l[others * 8 + g] = l[hg];
+                    }
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    *reinterpret_cast<float2*>(&merge_o[(warp * 8 + g) * 64 + n * 8 + 2 * t4]) = make_float2(o[hg][d0 / 8 + n][0], o[hg][d0 / 8 + n][1]);
+                    for (int i = 0; i < 4; ++i) {
+                        reinterpret_cast<float4*>(join_o)[(others * 4 + i) * 32 + lane] =
+                            make_float4(o[hg][d0 / 8 + 2 * i][0], o[hg][d0 / 8 + 2 * i][1], o[hg][d0 / 8 + 2 * i + 1][0], o[hg][d0 / 8 + 2 * i + 1][1]);
+                    }
                 }
                 __syncthreads();
-                for (int i = threadIdx.x; i < min(heads - hg * 8, 8) * 64; i += kThreads) {
-                    const int h = i / 64, d = d0 + i % 64;
-                    float mm = -INFINITY, ll = 0.f, v = 0.f;
+                if (warp == joiner) {
+                    float mm = m[hg], f[kWarps];
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, merge_m[w * 8 + h]);
+                    for (int w = 0; w < kWarps - 1; ++w) mm = fmaxf(mm, join_m[w * 8 + g]);
                     const float ref = mm == -INFINITY ? 0.f : mm;
+                    f[kWarps - 1] = exp2_fast(m[hg] - ref);
+                    float ll = l[hg] * f[kWarps - 1];
 #pragma unroll
-                    for (int w = 0; w < kWarps; ++w) {
-                        const float f = exp2f(merge_m[w * 8 + h] - ref);
-                        ll = fmaf(f, merge_l[w * 8 + h], ll);
-                        v = fmaf(f, merge_o[(w * 8 + h) * 64 + i % 64], v);
+                    for (int w = 0; w < kWarps - 1; ++w) {
+                        f[w] = exp2_fast(join_m[w * 8 + g] - ref);
+                        ll = fmaf(f[w], join_l[w * 8 + g], ll);
                     }
-                    const int row = hg * 8 + h;
-                    if (whole_item) {
-                        if (d < hd) static_cast<X*>(p.out)[(row0 + row) * hd + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
-                        if (d == 0 && p.lse != nullptr) p.lse[row0 + row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
-                    } else {
-                        part[32 + row * HD + d] = v;
-                        if (d == 0) {
+                    const int row = hg * 8 + g;
+                    const float norm = !whole_item ? 1.f : ll > 0.f ? 1.f / ll : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = o[hg][d0 / 8 + 2 * i + (e >> 1)][e & 1] * f[kWarps - 1];
+#pragma unroll
+                        for (int w = 0; w < kWarps - 1; ++w) {
+                            const float4 x = reinterpret_cast<const float4*>(join_o)[(w * 4 + i) * 32 + lane];
+                            v[0] = fmaf(f[w], x.x, v[0]);
+                            v[1] = fmaf(f[w], x.y, v[1]);
+                            v[2] = fmaf(f[w], x.z, v[2]);
+                            v[3] = fmaf(f[w], x.w, v[3]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int d = d0 + (2 * i + (e >> 1)) * 8 + 2 * t4 + (e & 1);
+                            if (row >= heads) continue;
+                            if (!whole_item) part[32 + row * HD + d] = v[e];
+                            else if (d < hd) static_cast<X*>(p.out)[(row0 + row) * hd + d] = from_float<X>(v[e] * norm);
+                        }
+                    }
+                    if (d0 == 0 && t4 == 0 && row < heads) {
+                        if (!whole_item) {
                             part[row] = mm;
                             part[16 + row] = ll;
+                        } else if (p.lse != nullptr) {
+                            p.lse[row0 + row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
                         }
                     }
                 }
             }
         }
-        if (!whole_item) {
-            // The item's CTAs are those of its flat tiles; the first one's counter tells who comes last.
-            const int c0 = static_cast<int>(seg.at / share), c1 = static_cast<int>((seg.at + seg.tiles - 1) / share);
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                __threadfence();
-                const unsigned n = atom_acq_rel_gpu_add(p.arrived + c0, 1u);
-                const bool last = n == static_cast<unsigned>(c1 - c0);
-                if (last) p.arrived[c0] = 0u;
-                shared_word[15] = last;
-                __threadfence();
-            }
-            __syncthreads();
-            if (shared_word[15]) join_parts<X, HD>(p, c0, c1, heads, row0, merge_o, merge_m);
+        if (seg.t0 != 0 && seg.t1 == seg.tiles && threadIdx.x == 0) {  // the item's CTAs are those of its flat tiles
+            const int c0 = static_cast<int>(seg.at / share);
+            p.endings[blockIdx.x] = {static_cast<int>(blockIdx.x) + 1 - c0, c0, heads, 0, row0};
         }
-        if (!next_segment<TILE>(p, walk, seg)) break;
-        __syncthreads();  // the joined values have been read
+        joiner = (joiner + 1) & (kWarps - 1);
+        if (!goes_on) break;
+        seg = following;
     }
     copy_wait<0>();
+}
+
+// Joins the partials of items that were cut, in the order of their CTAs: block c those of the item that ends in CTA c's first
+// segment. Several warps share a head's partials; the loads of each are independent of each other.
+constexpr int kJoinWarps = 16;
+template <typename X, int HD>
+__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Params p) {
+    constexpr int V = HD / 32;  // dims of a lane
+    __shared__ float warp_m[kJoinWarps], warp_l[kJoinWarps], warp_o[kJoinWarps][HD];
+    grid_dep_wait();
+    const int4 head = __ldcg(reinterpret_cast<const int4*>(p.endings + blockIdx.x));
+    if (head.x == 0) return;
+    const Ending e{head.x, head.y, head.z, 0, __ldcg(&p.endings[blockIdx.x].row0)};
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int ways = kJoinWarps / e.heads;  // warps of a head (16 heads at most)
+    const int h = warp / ways, way = warp % ways;
+    float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.f;
+    auto part = [&](int c) { return p.parts + (static_cast<size_t>(e.c0 + c) * 2 + (c == 0)) * kSlotFloats; };
+    if (h < e.heads) {
+        for (int from = way; from < e.n; from += 32 * ways) {
+            const int mine = from + lane * ways;
+            const float pm = mine < e.n ? __ldcg(part(mine) + h) : -INFINITY, pl = mine < e.n ? __ldcg(part(mine) + 16 + h) : 0.f;
+            float top = fmaxf(m, pm);
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float ref = top == -INFINITY ? 0.f : top, old = exp2_fast(m - ref), w = exp2_fast(pm - ref);
+            float sum = w * pl;
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            l = fmaf(l, old, sum);
+            m = top;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] *= old;
+            const int n = min(32, (e.n - from + ways - 1) / ways);
+#pragma unroll 8
+            for (int k = 0; k < n; ++k) {
+                const float* src = part(from + k * ways) + 32 + h * HD + lane * V;
+                const float f = __shfl_sync(0xffffffffu, w, k);
+                if constexpr (V == 2) {
+                    const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                    o[0] = fmaf(f, v.x, o[0]);
+                    o[1] = fmaf(f, v.y, o[1]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V / 4; ++i) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(src) + i);
+                        o[4 * i] = fmaf(f, v.x, o[4 * i]);
+                        o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
+                        o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]);
+                        o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
+                    }
+                }
+            }
+        }
+    }
+    if (lane == 0) {
+        warp_m[warp] = m;
+        warp_l[warp] = l;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) warp_o[warp][lane * V + i] = o[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < e.heads * HD; i += 32 * kJoinWarps) {
+        const int hh = i / HD, d = i % HD;
+        float mm = -INFINITY, ll = 0.f, v = 0.f;
+        for (int w = hh * ways; w < (hh + 1) * ways; ++w) mm = fmaxf(mm, warp_m[w]);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+        for (int w = hh * ways; w < (hh + 1) * ways; ++w) {
+            const float f = exp2_fast(warp_m[w] - ref);
+            ll = fmaf(f, warp_l[w], ll);
+            v = fmaf(f, warp_o[w][d], v);
+        }
+        const long long row = e.row0 + hh;
+        if (d < p.head_dim) static_cast<X*>(p.out)[row * p.head_dim + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
+        if (d == 0 && p.lse != nullptr) p.lse[row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
+    }
 }
 
 template <typename X, typename KV, int HD, int HG>
@@ -689,8 +789,8 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
     p.q = a.q;
     p.k = static_cast<const char*>(pg.k) + 2 * a.layer * pg.layer_stride;
     p.v = static_cast<const char*>(pg.v) + 2 * a.layer * pg.layer_stride;
-    p.parts = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kPagedCounterBytes);
-    p.arrived = static_cast<unsigned*>(a.workspace);
+    p.endings = static_cast<Ending*>(a.workspace);
+    p.parts = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + kEndingBytes);
     p.q_seq_stride = a.q_seq_stride;
     p.q_head_stride = a.q_head_stride;
     p.table_stride = a.table_stride;
@@ -708,6 +808,9 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
     p.per_head = (p.group + S::kHeads - 1) / S::kHeads;
     p.items = p.per_head * pg.n_kv_heads;
     p.page_div = fast_div(pg.page_size);
+    p.long_runs = pg.page_size % 16 == 0;
+    p.dense = pg.token_stride == HD && pg.head_dim == HD;
+    p.row_step = pg.token_stride * 2 * (32 / (HD / 8));
     auto kernel = attend_kernel<X, KV, HD, HG>;
     static std::atomic<uint64_t> allowed{0};  // devices on which this kernel may use its shared memory
     int dev = 0;
@@ -728,11 +831,12 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
         p.out = static_cast<X*>(a.out) + static_cast<long long>(b0) * a.n_heads * pg.head_dim;
         p.lse = a.lse != nullptr ? a.lse + static_cast<long long>(b0) * a.n_heads : nullptr;
         const size_t smem = S::kFixed + 4 * (static_cast<size_t>(p.n_seq) + 1);
-        const int per_sm = smem <= 113 * 1024 ? 2 : 1;
-        const long long most = std::max<long long>(1, (row_tiles + kWarps - 1) / kWarps * p.n_seq + p.items * static_cast<long long>(p.n_seq));
-        const int grid = static_cast<int>(std::min<long long>(std::min(kMaxCtas, num_sms() * per_sm), most));
-        kernel<<<grid, kThreads, smem, stream>>>(p);
-        CLLM_CUDA(cudaGetLastError());
+        const long long most = std::max<long long>(1, (row_tiles + kUnit - 1) / kUnit * p.n_seq + p.items * static_cast<long long>(p.n_seq));
+        const int grid = static_cast<int>(std::min<long long>(std::min(kMaxCtas, num_sms() * std::min(S::kCtas, static_cast<int>(228 * 1024 / (smem + 1024)))), most));
+        launch_kernel(kernel, dim3(grid), dim3(kThreads), smem, stream, false, p);
+        // Items of up to kUnit tiles are cut only where equal shares cut them, which takes more tiles than there are CTAs x kUnit.
+        const bool can_cut = (cap + S::kTile - 1) / S::kTile > kUnit || static_cast<long long>(p.n_seq) * p.items > grid;
+        if (can_cut) launch_kernel(join_kernel<X, HD>, dim3(grid), dim3(32 * kJoinWarps), 0, stream, true, p);
     }
 }
 
@@ -750,7 +854,7 @@ void launch_types(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
 
 }  // namespace
 
-size_t attend_workspace_bytes() { return kPagedCounterBytes + sizeof(float) * kSlotFloats * 2 * kMaxCtas; }
+size_t attend_workspace_bytes() { return kEndingBytes + sizeof(float) * kSlotFloats * 2 * kMaxCtas; }
 
 void launch_paged_attend(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStream_t stream) {
     if (a.n_seq == 0) return;

@@ -223,8 +223,8 @@ int cudallm_beam_select(const cudallm_beam_args* a, void* stream) {
         CLLM_REQUIRE(a != nullptr && a->struct_size == static_cast<int>(sizeof(cudallm_beam_args)),
                      "cudallm_beam_args.struct_size must be sizeof(cudallm_beam_args)");
         check_x_dtype(a->x_dtype);
-        CLLM_REQUIRE(a->beams >= 1 && a->beams <= kMaxBeams && a->keep >= 1 && a->keep <= kMaxKeep && a->vocab >= 1,
-                     "beams and keep must be in 1 .. 64, vocab positive");
+        CLLM_REQUIRE(a->beams >= 1 && a->beams <= kMaxBeams && a->keep >= 1 && a->keep <= kMaxKeep && a->vocab >= 1 && a->vocab <= kMaxVocab,
+                     "beams and keep must be in 1 .. 64, vocab in 1 .. 2^24");
         CLLM_REQUIRE(a->keep <= static_cast<long long>(a->beams) * a->vocab, "keep must be at most beams * vocab");
         CLLM_REQUIRE(a->n_groups >= 0 && static_cast<long long>(a->n_groups) * a->beams <= kMaxPageRows, "n_groups * beams must be in 0 .. 65536");
         if (a->n_groups == 0) return;

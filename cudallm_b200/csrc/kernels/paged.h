@@ -11,10 +11,9 @@
 
 namespace cudallm {
 
-// The first bytes of every workspace hold counters that are zero between calls; the rest is scratch.
-constexpr size_t kPagedCounterBytes = CUDALLM_WORKSPACE_COUNTERS;
 constexpr int kMaxBeams = 64;
 constexpr int kMaxKeep = 64;
+constexpr int kMaxVocab = 1 << 24;
 constexpr int kMaxPageRows = 65536;
 
 void launch_paged_attend(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStream_t stream);

@@ -49,7 +49,7 @@ struct ForkScratch {
 };
 
 __host__ __device__ inline ForkScratch fork_scratch(void* workspace, int rows) {
-    int* p = reinterpret_cast<int*>(static_cast<char*>(workspace) + kPagedCounterBytes);
+    int* p = static_cast<int*>(workspace);
     ForkScratch s;
     s.n_found = p;
     p += 64;
@@ -198,7 +198,7 @@ struct CompactScratch {
 };
 
 __host__ __device__ inline CompactScratch compact_scratch(void* workspace, int n_pages) {
-    int* p = reinterpret_cast<int*>(static_cast<char*>(workspace) + kPagedCounterBytes);
+    int* p = static_cast<int*>(workspace);
     CompactScratch s;
     s.n_moves = p;
     p += 64;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(cudallm_page
 size_t pages_workspace_bytes(int n_pages, int rows) {
     if (n_pages < 1 || rows < 0 || rows > kMaxPageRows) return 0;
     const size_t fork = 6 * static_cast<size_t>(rows) + n_pages, compact = 3 * static_cast<size_t>(n_pages);
-    return kPagedCounterBytes + 4 * (64 + (fork > compact ? fork : compact));
+    return 4 * (64 + (fork > compact ? fork : compact));
 }
 
 void launch_paged_fork(const cudallm_pages& pg, const cudallm_fork_args& a, cudaStream_t stream) {

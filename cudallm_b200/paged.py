@@ -30,7 +30,6 @@ __all__ = ["PagedCache", "Rope", "beam_select"]
 _X = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _KV = {torch.float16: 0, torch.bfloat16: 1}
 _INVALID_ARG = 1
-_COUNTERS = 16 * 1024  # leading bytes of a workspace that a call expects, and leaves, at zero
 
 
 def _refuse(message: str):
@@ -50,20 +49,18 @@ def _args(name: str):
 
 
 class _Workspaces:
-    """Workspaces of a device's streams, whose counters start at zero (calls on different streams may overlap)."""
+    """A workspace for each of a device's streams (calls on different streams may overlap)."""
 
     def __init__(self, device: torch.device):
         self.device = device
         self.by_stream: dict[int, torch.Tensor] = {}
 
     def get(self, stream: int, size: int) -> torch.Tensor:
-        capturing = torch.cuda.is_current_stream_capturing()
-        w = None if capturing else self.by_stream.get(stream)
+        if torch.cuda.is_current_stream_capturing():  # the graph's own, which later calls must not replace
+            return torch.empty(size, dtype=torch.uint8, device=self.device)
+        w = self.by_stream.get(stream)
         if w is None or w.numel() < size:
-            w = torch.empty(size, dtype=torch.uint8, device=self.device)
-            w[:_COUNTERS].zero_()
-            if not capturing:  # one made during a capture belongs to the graph, which zeroes its counters at every replay
-                self.by_stream[stream] = w
+            w = self.by_stream[stream] = torch.empty(size, dtype=torch.uint8, device=self.device)
         return w
 
 

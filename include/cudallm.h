@@ -250,11 +250,8 @@ int cudallm_attention_noalloc(const float* q, const unsigned short* k_cache, con
  * What the host cannot see (lengths, tables, positions, parents) is bounded inside the kernels as stated below,
  * so no content of those arrays leads to an access outside of the caller's buffers.
  *
- * Workspaces: `workspace` points to at least cudallm_*_workspace_bytes() bytes, 256-byte aligned, whose first
- * CUDALLM_WORKSPACE_COUNTERS bytes the caller sets to zero once, when it is allocated; every call leaves them zero. A workspace may serve
+ * Workspaces: `workspace` points to at least cudallm_*_workspace_bytes() bytes, 256-byte aligned; its contents do not matter. One may serve
  * all of these calls, one after the other on one stream; calls that may overlap (other streams) need their own. */
-
-#define CUDALLM_WORKSPACE_COUNTERS 16384
 
 #define CUDALLM_X_FP32 0
 #define CUDALLM_X_FP16 1
@@ -380,7 +377,7 @@ unsigned long long cudallm_pages_workspace_bytes(int n_pages, int rows);
  * w of logits, or, where finished[g][w] != 0 (finished may be NULL), x = 0 at eos and -inf elsewhere. A candidate that
  * is not a number counts as -inf. The `keep` best of each group, in order: larger candidate, then lower beam, then
  * larger logit (one that is not a number: -inf), then lower token. out_parents are rows of logits (as
- * cudallm_paged_fork takes them). beams 1 .. 64, keep 1 .. 64 and at most beams * vocab. */
+ * cudallm_paged_fork takes them). beams 1 .. 64, keep 1 .. 64 and at most beams * vocab, vocab at most 2^24. */
 typedef struct {
     int struct_size; /* sizeof(cudallm_beam_args) */
     int x_dtype, n_groups, beams, keep, vocab, eos, reserved;

@@ -117,11 +117,10 @@ def test_beam_refusals(native_lib, over):
 def test_messages_and_workspace_sizes(native_lib):
     assert _refused(native_lib, "cudallm_paged_attend", _pages(), _attend(layer=7))
     assert b"layer" in native_lib.cudallm_last_error()
-    counters = 16384
-    assert native_lib.cudallm_attend_workspace_bytes() >= counters
-    assert native_lib.cudallm_pages_workspace_bytes(1000, 64) > counters
+    assert native_lib.cudallm_attend_workspace_bytes() > 0
+    assert native_lib.cudallm_pages_workspace_bytes(1000, 64) > 4000
     assert native_lib.cudallm_pages_workspace_bytes(0, 64) == 0 and native_lib.cudallm_pages_workspace_bytes(8, 1 << 20) == 0
-    assert native_lib.cudallm_beam_workspace_bytes(64, 128256, 16) > counters and native_lib.cudallm_beam_workspace_bytes(4, 100, 65) == 0
+    assert native_lib.cudallm_beam_workspace_bytes(64, 128256, 16) > 64 * 16 * 8 and native_lib.cudallm_beam_workspace_bytes(4, 100, 65) == 0
 
 
 def test_tensors_off_the_gpu_are_refused():

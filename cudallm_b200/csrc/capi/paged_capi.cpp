@@ -146,6 +146,7 @@ int cudallm_paged_append(const cudallm_pages* pages, const cudallm_append_args* 
         CLLM_REQUIRE(a->q_token_stride >= 0 && a->q_head_stride >= 0 && a->k_token_stride >= 0 && a->k_head_stride >= 0 &&
                          a->v_token_stride >= 0 && a->v_head_stride >= 0,
                      "strides must not be negative");
+        CLLM_REQUIRE(a->n_heads <= 65536 && pages->n_kv_heads <= 65536, "at most 65536 heads");
         if (a->q != nullptr) {
             const long long T = a->n_tokens, H = a->n_heads, hd = pages->head_dim, ts = a->out_token_stride, hs = a->out_head_stride;
             const bool token_outer = (H == 1 || hs >= hd) && (T == 1 || ts >= (H == 1 ? hd : hs * (H - 1) + hd));

@@ -50,19 +50,6 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr size_t kEndingBytes = 32 * kMaxCtas;
 constexpr int kUnit = 8;  // tiles of a CTA where there are few
 
-// n / d for 0 <= n < 2^31 as a multiplication.
-struct FastDiv {
-    unsigned mul, shift;
-};
-FastDiv fast_div(int d) {
-    unsigned s = 0;
-    while ((1u << s) < static_cast<unsigned>(d)) ++s;
-    return {static_cast<unsigned>(((1ull << (31 + s)) + d - 1) / d), 31 + s};
-}
-__device__ __forceinline__ int div_by(int n, FastDiv f) {
-    return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(n)) * f.mul) >> f.shift);
-}
-
 // What a CTA's first segment is the last part of: the partials of CTAs c0 .. c0 + n - 1 make up `heads` rows of the output (n = 0: nothing).
 struct __align__(16) Ending {
     int n, c0, heads, pad;

@@ -1,4 +1,4 @@
-// Device helpers shared by the paged-cache kernels: element conversion and page lookup.
+// Helpers shared by the paged-cache kernels: element conversion, division by a constant of the launch.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -25,6 +25,19 @@ __device__ __forceinline__ __half from_float<__half>(float v) {
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) {
     return __float2bfloat16_rn(v);
+}
+
+// n / d for 0 <= n < 2^31 as a multiplication.
+struct FastDiv {
+    unsigned mul, shift;
+};
+inline FastDiv fast_div(int d) {
+    unsigned s = 0;
+    while ((1u << s) < static_cast<unsigned>(d)) ++s;
+    return {static_cast<unsigned>(((1ull << (31 + s)) + d - 1) / d), 31 + s};
+}
+__device__ __forceinline__ int div_by(int n, FastDiv f) {
+    return static_cast<int>((static_cast<unsigned long long>(static_cast<unsigned>(n)) * f.mul) >> f.shift);
 }
 
 }  // namespace cudallm

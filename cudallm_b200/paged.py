@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -26,6 +27,12 @@ from . import abi
 from .abi import CudaLLMError, check, lib
 
 __all__ = ["PagedCache", "Rope", "beam_select"]
+
+try:  # a tenth of the time of torch.cuda.current_stream
+    from torch._C import _cuda_getCurrentRawStream as _stream_of
+except ImportError:
+    def _stream_of(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
 
 _X = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _KV = {torch.float16: 0, torch.bfloat16: 1}
@@ -46,6 +53,16 @@ def _args(name: str):
     a = abi.struct(name)()
     a.struct_size = ctypes.sizeof(a)
     return a, ctypes.byref(a)
+
+
+_beam = threading.local()
+
+
+def _beam_args():
+    """This thread's argument struct of beam_select."""
+    if not hasattr(_beam, "args"):
+        _beam.args = _args("cudallm_beam_args")
+    return _beam.args
 
 
 class _Workspaces:
@@ -155,6 +172,7 @@ class PagedCache:
               "k and v must be fp16 or bf16 tensors [layers][pages][kv heads][page size][head dim] of one shape on one GPU")
         _need(k.stride() == v.stride() and k.stride(4) == 1, "k and v must have the same strides, and a head's dims side by side")
         self.k, self.v, self.device = k, v, k.device
+        self._index = k.device.index
         self.n_layers, self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         p, self._pages = _args("cudallm_pages")
         p.kv_dtype = _KV[k.dtype]
@@ -162,6 +180,8 @@ class PagedCache:
         p.k, p.v = k.data_ptr(), v.data_ptr()
         p.layer_stride, p.page_stride, p.head_stride, p.token_stride = k.stride()[:4]
         self._lib = lib()
+        self._call_attend, self._call_append = self._lib.cudallm_paged_attend, self._lib.cudallm_paged_append
+        self._call_fork, self._call_compact = self._lib.cudallm_paged_fork, self._lib.cudallm_paged_compact
         self._attend, self._attend_ref = _args("cudallm_attend_args")
         self._append, self._append_ref = _args("cudallm_append_args")
         self._fork, self._fork_ref = _args("cudallm_fork_args")
@@ -181,17 +201,17 @@ class PagedCache:
         new = lambda shape, v: torch.full(shape, v, dtype=torch.int32, device=self.device)  # noqa: E731
         return new((n, width), -1), new((n,), 0), new((self.n_pages,), 0)
 
-    def _run(self, fn, args_ref) -> None:
-        index = self.device.index
-        stream = torch.cuda.current_stream(index).cuda_stream
-        if torch.cuda.current_device() == index:
-            check(fn(self._pages, args_ref, stream))
+    def _run(self, fn, args_ref, stream: int) -> None:
+        if torch.cuda.current_device() == self._index:
+            rc = fn(self._pages, args_ref, stream)
         else:
-            with _OnDevice(index):
-                check(fn(self._pages, args_ref, stream))
+            with _OnDevice(self._index):
+                rc = fn(self._pages, args_ref, stream)
+        if rc:
+            check(rc)
 
-    def _workspace(self, a, size: int):
-        w = self._workspaces.get(torch.cuda.current_stream(self.device.index).cuda_stream, size)
+    def _workspace(self, a, size: int, stream: int):
+        w = self._workspaces.get(stream, size)
         a.workspace, a.workspace_bytes = w.data_ptr(), w.numel()
         return w
 
@@ -210,17 +230,18 @@ class PagedCache:
         a = self._attend
         a.lens = _int32(lens, self.device, (n,), "lens")
         if out is None:
-            out = torch.empty((n, heads, self.head_dim), dtype=q.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.dtype is not q.dtype or out.device != self.device or out.shape != q.shape or not out.is_contiguous():
             _refuse("out must be contiguous, with q's shape and type")
-        lse = torch.empty((n, heads), dtype=torch.float32, device=self.device) if with_lse else None
+        lse = q.new_empty((n, heads), dtype=torch.float32) if with_lse else None
         a.layer, a.x_dtype, a.n_seq, a.n_heads, a.table_width, a.window = layer, x, n, heads, width, window
         a.scale = self.head_dim ** -0.5 if scale is None else scale
         a.q, a.q_seq_stride, a.q_head_stride = q.data_ptr(), a_seq, a_head
         a.tables, a.table_stride, a.out = tables.data_ptr(), stride, out.data_ptr()
         a.lse = None if lse is None else lse.data_ptr()
-        keep = self._workspace(a, self._attend_bytes)  # noqa: F841  lives until the launch
-        self._run(self._lib.cudallm_paged_attend, self._attend_ref)
+        stream = _stream_of(self._index)
+        keep = self._workspace(a, self._attend_bytes, stream)  # noqa: F841  lives until the launch
+        self._run(self._call_attend, self._attend_ref, stream)
         return (out, lse) if with_lse else out
 
     def append(self, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, tables: torch.Tensor,
@@ -244,7 +265,7 @@ class PagedCache:
             if nq != n:
                 _refuse("q, k and v must have the same number of tokens")
             if out is None:
-                out = torch.empty((n, heads, dim), dtype=q.dtype, device=dev)
+                out = torch.empty_like(q, memory_format=torch.contiguous_format)
             elif out.shape != q.shape:
                 _refuse("out must have q's shape")
             _, _, a.out_token_stride, a.out_head_stride = _heads(out, dev, k.dtype, dim, "out")
@@ -261,7 +282,7 @@ class PagedCache:
                 _refuse("the rotation's frequencies must be on the cache's device")
             a.rotary, a.interleaved, a.factor, a.inv_freq = rope.rotary, rope.interleaved, rope.factor, rope.inv_freq.data_ptr()
         a.k, a.v, a.tables, a.table_stride = k.data_ptr(), v.data_ptr(), tables.data_ptr(), stride
-        self._run(self._lib.cudallm_paged_append, self._append_ref)
+        self._run(self._call_append, self._append_ref, _stream_of(self._index))
         return out
 
     def fork(self, tables: torch.Tensor, lens: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor, *, room: int = 1,
@@ -277,9 +298,7 @@ class PagedCache:
         a.refs = _int32(refs, dev, (self.n_pages,), "refs")
         a.parents = _int32(parents, dev, (n_out,), "parents")
         if out is None:
-            new = torch.empty(n_out * width + n_out + self.n_pages + 1, dtype=torch.int32, device=dev)
-            t, n, r, missing = new.split([n_out * width, n_out, self.n_pages, 1])
-            out = (t.view(n_out, width), n, r, missing)
+            out = (tables.new_empty((n_out, width)), torch.empty_like(parents), torch.empty_like(refs), refs.new_empty(1))
         t_rows, t_width, a.table_out_stride = _table(out[0], dev, "out tables")
         if t_rows != n_out or t_width != width:
             _refuse(f"out tables must be [{n_out}][{width}]")
@@ -288,8 +307,9 @@ class PagedCache:
         a.missing = _int32(out[3], dev, (1,), "missing")
         a.n_rows, a.n_out, a.table_width, a.room = n_rows, n_out, width, room
         a.tables, a.tables_out = tables.data_ptr(), out[0].data_ptr()
-        keep = self._workspace(a, self._lib.cudallm_pages_workspace_bytes(self.n_pages, max(n_rows, n_out)))  # noqa: F841
-        self._run(self._lib.cudallm_paged_fork, self._fork_ref)
+        stream = _stream_of(self._index)
+        keep = self._workspace(a, self._lib.cudallm_pages_workspace_bytes(self.n_pages, max(n_rows, n_out)), stream)  # noqa: F841
+        self._run(self._call_fork, self._fork_ref, stream)
         return out
 
     def compact(self, tables: torch.Tensor, refs: torch.Tensor, *, out: tuple | None = None):
@@ -299,9 +319,7 @@ class PagedCache:
         n_rows, width, a.table_stride = _table(tables, dev, "tables")
         a.refs = _int32(refs, dev, (self.n_pages,), "refs")
         if out is None:
-            new = torch.empty(n_rows * width + self.n_pages + 1, dtype=torch.int32, device=dev)
-            t, r, live = new.split([n_rows * width, self.n_pages, 1])
-            out = (t.view(n_rows, width), r, live)
+            out = (tables.new_empty((n_rows, width)), torch.empty_like(refs), refs.new_empty(1))
         t_rows, t_width, a.table_out_stride = _table(out[0], dev, "out tables")
         if t_rows != n_rows or t_width != width:
             _refuse(f"out tables must be [{n_rows}][{width}]")
@@ -309,8 +327,9 @@ class PagedCache:
         a.live = _int32(out[2], dev, (1,), "live")
         a.n_rows, a.table_width = n_rows, width
         a.tables, a.tables_out = tables.data_ptr(), out[0].data_ptr()
-        keep = self._workspace(a, self._lib.cudallm_pages_workspace_bytes(self.n_pages, n_rows))  # noqa: F841
-        self._run(self._lib.cudallm_paged_compact, self._compact_ref)
+        stream = _stream_of(self._index)
+        keep = self._workspace(a, self._lib.cudallm_pages_workspace_bytes(self.n_pages, n_rows), stream)  # noqa: F841
+        self._run(self._call_compact, self._compact_ref, stream)
         return out
 
 
@@ -331,11 +350,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     row_stride, inner = logits.stride()
     if rows != groups * beams or (rows and vocab > 1 and inner != 1):
         _refuse("logits must have groups * beams rows with their values side by side")
-    a, ref = _args("cudallm_beam_args")
+    a, ref = _beam_args()
     a.finished = None if finished is None else _int32(finished, dev, (groups, beams), "finished")
     if out is None:
-        new = torch.empty((3, groups, keep), dtype=torch.int32, device=dev)
-        out = (new[0].view(torch.float32), new[1], new[2])
+        out = (scores.new_empty((groups, keep)), *torch.empty((2, groups, keep), dtype=torch.int32, device=dev).unbind(0))
     elif out[0].dtype is not torch.float32 or out[0].device != dev or tuple(out[0].shape) != (groups, keep) or not out[0].is_contiguous():
         _refuse("out scores must be a contiguous fp32 tensor [groups][keep]")
     a.out_scores = out[0].data_ptr()
@@ -345,9 +363,17 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     a.logits, a.row_stride, a.scores = logits.data_ptr(), row_stride, scores.data_ptr()
     L = lib()
     index = dev.index
-    stream = torch.cuda.current_stream(index).cuda_stream
-    w = _shared.setdefault(index, _Workspaces(dev)).get(stream, L.cudallm_beam_workspace_bytes(rows, vocab, keep))
+    stream = _stream_of(index)
+    spaces = _shared.get(index)
+    if spaces is None:
+        spaces = _shared[index] = _Workspaces(dev)
+    w = spaces.get(stream, L.cudallm_beam_workspace_bytes(rows, vocab, keep))
     a.workspace, a.workspace_bytes = w.data_ptr(), w.numel()
-    with _OnDevice(index):
-        check(L.cudallm_beam_select(ref, stream))
+    if torch.cuda.current_device() == index:
+        rc = L.cudallm_beam_select(ref, stream)
+    else:
+        with _OnDevice(index):
+            rc = L.cudallm_beam_select(ref, stream)
+    if rc:
+        check(rc)
     return out

@@ -8,6 +8,7 @@
 // Where strides or sizes do not allow that, a unit is one pair or one dim.
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 
 #include "common/check.h"
 #include "kernels/kernels.h"
@@ -21,7 +22,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kTokens = 8;  // of a block at most
-constexpr int kBatch = 3;   // units of a thread that are loaded together
 
 struct Params {
     cudallm_pages pg;
@@ -29,8 +29,29 @@ struct Params {
     int q_heads, heads;   // query heads; all heads of a token
     int tokens;           // of a block
     int pairs, pair_units, units;  // rotated pairs of a head; its units that rotate; all its units
-    FastDiv by_units, by_heads;
 };
+
+// 8 values of a 16-byte (or two) word and back.
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4 (&raw)[sizeof(T) / 2], float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+        memcpy(v, raw, 32);
+    } else {
+        const uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                __half2 h;
+                memcpy(&h, &w[i], 4);
+                v[2 * i] = __low2float(h);
+                v[2 * i + 1] = __high2float(h);
+            } else {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+}
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
@@ -38,12 +59,18 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
         *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
         *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-        T x[8];
+        uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = from_float<T>(v[i]);
-        uint4 raw;
-        memcpy(&raw, x, 16);
-        *reinterpret_cast<uint4*>(p) = raw;
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (std::is_same_v<T, __half>) {
+                const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                memcpy(&w[i], &h, 4);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                memcpy(&w[i], &h, 4);
+            }
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -53,86 +80,95 @@ __device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
     a = x;
 }
 
-// A unit of a head as its source holds it: 8 dims, or two times 8 (16-byte words); or one dim, or two.
-template <typename X, bool WIDE>
-struct Unit {
-    uint4 raw[WIDE ? sizeof(X) : 1];
-    X one[2];
+// How heads are cut into units.
+enum class Layout {
+    kHalves,       // 8 pairs (j, j + n): two words of 8 dims; copied dims: one word
+    kInterleaved,  // 4 pairs (2j, 2j + 1) or 8 copied dims: one word
+    kSingle,       // one pair of either kind, or one copied dim
 };
 
-// Dims of unit u: the first ones, and the second ones where it has two parts.
-template <bool WIDE>
-__device__ __forceinline__ void places(const Params& p, int u, bool& pair, int& d0, int& d1) {
-    constexpr int kDims = WIDE ? 8 : 1;
-    pair = u < p.pair_units;
-    const bool halves = pair && !p.a.interleaved;
-    d0 = pair ? u * kDims : 2 * p.pairs + (u - p.pair_units) * kDims;
-    if (!WIDE && pair && p.a.interleaved) d0 = 2 * u;
-    d1 = halves ? d0 + p.pairs : !WIDE && pair ? d0 + 1 : -1;
-}
+// What a thread does in every head: its dims from d0 on and, `other` dims further, its second part if it has one; the cosines and sines
+// of the pairs that it rotates, if it does.
+template <Layout L>
+struct Job {
+    static constexpr int kPairs = L == Layout::kHalves ? 8 : L == Layout::kInterleaved ? 4 : 1;
+    int other;
+    bool pair, two;
+    float c[kPairs], s[kPairs];
+};
 
-template <typename X, bool WIDE>
-__device__ __forceinline__ void read_unit(const Params& p, int u, const X* src, Unit<X, WIDE>& r) {
-    bool pair;
-    int d0, d1;
-    places<WIDE>(p, u, pair, d0, d1);
-    if constexpr (WIDE) {
-        constexpr int kWords = sizeof(X) / 2;  // of 8 dims
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) {
-            r.raw[i] = reinterpret_cast<const uint4*>(src + d0)[i];
-            if (d1 >= 0) r.raw[kWords + i] = reinterpret_cast<const uint4*>(src + d1)[i];
-        }
-    } else {
-        r.one[0] = src[d0];
-        if (d1 >= 0) r.one[1] = src[d1];
-    }
-}
+// One unit as it is loaded.
+template <typename X, Layout L>
+struct Unit {
+    static constexpr int kWords = L == Layout::kSingle ? 1 : sizeof(X) / 2;  // of 8 dims
+    uint4 a[kWords], b[kWords];
+    X one[2];
 
-// Rotates a unit and stores it. cos and sin are the token's.
-template <typename X, typename Y, bool WIDE>
-__device__ __forceinline__ void write_unit(const Params& p, int u, bool rotates, bool clear, const Unit<X, WIDE>& r, Y* dst, const float* cos, const float* sin) {
-    bool pair;
-    int d0, d1;
-    places<WIDE>(p, u, pair, d0, d1);
-    if constexpr (WIDE) {
-        constexpr int kWords = sizeof(X) / 2;
-        X x[16];
-        memcpy(x, r.raw, sizeof(X) * 16);
-        float v[8], w[8];
+    __device__ __forceinline__ void load(const Job<L>& w, const X* src) {
+        if constexpr (L == Layout::kSingle) {
+            one[0] = src[0];
+            if (w.two) one[1] = src[w.other];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            v[i] = as_float(x[i]);
-            w[i] = as_float(x[8 + i]);
-        }
-        if (d1 >= 0) {
-            if (rotates) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) turn(v[i], w[i], cos[d0 + i], sin[d0 + i]);
+            for (int i = 0; i < kWords; ++i) {
+                a[i] = reinterpret_cast<const uint4*>(src)[i];
+                if (L == Layout::kHalves && w.two) b[i] = reinterpret_cast<const uint4*>(src + w.other)[i];
             }
-        } else if (pair && rotates) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) turn(v[2 * i], v[2 * i + 1], cos[u * 4 + i], sin[u * 4 + i]);
         }
-        if (clear) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = w[i] = 0.f;
-        }
-        store8(dst + d0, v);
-        if (d1 >= 0) store8(dst + d1, w);
-        static_assert(sizeof(r.raw) == 2 * kWords * 16, "two times 8 dims");
-    } else {
-        float a = as_float(r.one[0]), b = d1 >= 0 ? as_float(r.one[1]) : 0.f;
-        if (pair && rotates) turn(a, b, cos[u], sin[u]);
-        if (clear) a = b = 0.f;
-        dst[d0] = from_float<Y>(a);
-        if (d1 >= 0) dst[d1] = from_float<Y>(b);
     }
-}
 
-template <typename X, typename KV, bool WIDE>
-__global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant__ Params p) {
-    __shared__ float cos[kTokens][128], sin[kTokens][128];
+    // Rotated if `rotates`.
+    template <typename Y>
+    __device__ __forceinline__ void store(const Job<L>& w, bool rotates, Y* dst) const {
+        rotates = rotates && w.pair;
+        if constexpr (L == Layout::kSingle) {
+            float v = as_float(one[0]), z = w.two ? as_float(one[1]) : 0.f;
+            if (rotates) turn(v, z, w.c[0], w.s[0]);
+            dst[0] = from_float<Y>(v);
+            if (w.two) dst[w.other] = from_float<Y>(z);
+        } else if (std::is_same_v<X, Y> && !rotates) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                reinterpret_cast<uint4*>(dst)[i] = a[i];
+                if (L == Layout::kHalves && w.two) reinterpret_cast<uint4*>(dst + w.other)[i] = b[i];
+            }
+        } else {
+            float v[8];
+            unpack8<X>(a, v);
+            if (L == Layout::kHalves && w.two) {
+                float z[8];
+                unpack8<X>(b, z);
+                if (rotates) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) turn(v[i], z[i], w.c[i % Job<L>::kPairs], w.s[i % Job<L>::kPairs]);
+                }
+                store8(dst + w.other, z);
+            }
+            if (L == Layout::kInterleaved && rotates) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) turn(v[2 * i], v[2 * i + 1], w.c[i % Job<L>::kPairs], w.s[i % Job<L>::kPairs]);
+            }
+            store8(dst, v);
+        }
+    }
+
+    __device__ __forceinline__ void clear() {
+        one[0] = one[1] = from_float<X>(0.f);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) a[i] = b[i] = make_uint4(0, 0, 0, 0);
+    }
+};
+
+// Units of 8 pairs or of fp32 are loaded one at a time, by 4 blocks on an SM; smaller ones two at a time, by 5. Measured on 16383 tokens (us):
+// bf16, 48 heads of 128 dims, 64 of them rotated interleaved: 4 loads and 3 blocks 91, 2 and 5 81, 1 and 5 84; all rotated in halves: 2 and 3
+// 80, 2 and 4 110 (spills), 1 and 4 80; fp32, 64 dims in halves: 2 and 3 109, 1 and 4 70.
+template <typename X, Layout L>
+constexpr bool few_registers = L == Layout::kHalves || (L == Layout::kInterleaved && sizeof(X) == 4);
+
+template <typename X, typename KV, Layout L>
+__global__ void __launch_bounds__(kThreads, few_registers<X, L> ? 4 : 5) append_kernel(const __grid_constant__ Params p) {
+    constexpr int kItems = few_registers<X, L> ? 1 : 2;  // heads of a thread whose loads are under way together
+    __shared__ __align__(16) float cos[kTokens][128], sin[kTokens][128];
     __shared__ long long slots[kTokens];  // where the token's keys go; -1: nowhere, -2: padding
     const cudallm_append_args& a = p.a;
     const int first = blockIdx.x * p.tokens, tokens = min(p.tokens, a.n_tokens - first);
@@ -154,39 +190,80 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const __grid_constant_
         cos[t][k] = c * a.factor;
         sin[t][k] = s * a.factor;
     }
-    // The heads' loads are under way before the block waits for its cosines and slots.
-    const int total = tokens * p.heads * p.units, step = gridDim.y * kThreads;
-    bool waited = false;
-    for (int x0 = blockIdx.y * kThreads + threadIdx.x; x0 < total || !waited; x0 += kBatch * step) {
-        Unit<X, WIDE> units[kBatch];
+    // A thread has the same dims in all of its heads; at_once heads side by side, of several tokens where a token has fewer.
+    // Units that rotate and units that are copied go to different warps.
+    const int at_once = kThreads / p.units, turning = at_once * p.pair_units, copying = p.units - p.pair_units;
+    const int place = static_cast<int>(threadIdx.x) - turning;
+    const int u = place < 0 ? threadIdx.x % p.pair_units : copying > 0 ? p.pair_units + place % copying : p.units;
+    const int r = place < 0 ? threadIdx.x / p.pair_units : copying > 0 ? place / copying : at_once;
+    const int together = gridDim.y > 1 ? 1 : max(1, at_once / p.heads);  // tokens
+    const int step = together > 1 ? p.heads : gridDim.y * at_once;
+    const int h0 = together > 1 ? r % p.heads : blockIdx.y * at_once + r;  // the thread's first head
+    int t0 = together > 1 ? r / p.heads : 0;
+    if (t0 >= together || r >= at_once) t0 = tokens;
+    Job<L> w;
+    w.pair = u < p.pair_units;
+    const int copied = 2 * p.pairs + (u - p.pair_units) * (L == Layout::kSingle ? 1 : 8);
+    const int d0 = !w.pair ? copied : L != Layout::kSingle ? u * 8 : a.interleaved ? u * 2 : u;
+    w.two = w.pair && L != Layout::kInterleaved;
+    w.other = L == Layout::kSingle && a.interleaved ? 1 : p.pairs;
+    const int kv = p.pg.n_kv_heads;
+    __syncthreads();
+#pragma unroll 1
+    for (int hs = h0; hs < p.heads; hs += kItems * step) {
+        // Up to kItems heads, the same ones of every token.
+        const X* src[kItems];
+        long long ahead[kItems];  // from a token's source to the next one's
+        X* out[kItems];           // of queries
+        KV* page[kItems];         // of keys and values: plus the token's slot
+        bool rotates[kItems];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int x = x0 + k * step;
-            if (x >= total) break;
-            const int hh = div_by(x, p.by_units), t = div_by(hh, p.by_heads), head = hh - t * p.heads;
-            const long long i = first + t;
-            const int kvh = head - p.q_heads;
-            const X* src = kvh < 0                 ? static_cast<const X*>(a.q) + i * a.q_token_stride + head * a.q_head_stride
-                           : kvh < p.pg.n_kv_heads ? static_cast<const X*>(a.k) + i * a.k_token_stride + kvh * a.k_head_stride
-                                                   : static_cast<const X*>(a.v) + i * a.v_token_stride + (kvh - p.pg.n_kv_heads) * a.v_head_stride;
-            read_unit<X, WIDE>(p, x - hh * p.units, src, units[k]);
+        for (int j = 0; j < kItems; ++j) {
+            const int h = hs + j * step, kh = h - p.q_heads, vh = kh - kv;
+            out[j] = nullptr;
+            page[j] = nullptr;
+            rotates[j] = vh < 0;
+            if (kh < 0) {
+                ahead[j] = a.q_token_stride;
+                src[j] = static_cast<const X*>(a.q) + h * a.q_head_stride;
+                out[j] = static_cast<X*>(a.q_out) + (first + t0) * a.out_token_stride + h * a.out_head_stride + d0;
+            } else if (vh < 0) {
+                ahead[j] = a.k_token_stride;
+                src[j] = static_cast<const X*>(a.k) + kh * a.k_head_stride;
+                page[j] = static_cast<KV*>(p.pg.k) + kh * p.pg.head_stride + d0;
+            } else {
+                ahead[j] = a.v_token_stride;
+                src[j] = static_cast<const X*>(a.v) + vh * a.v_head_stride;
+                page[j] = static_cast<KV*>(p.pg.v) + vh * p.pg.head_stride + d0;
+            }
+            src[j] = vh < kv ? src[j] + (first + t0) * ahead[j] + d0 : nullptr;
+            ahead[j] *= together;
         }
-        if (!waited) __syncthreads();
-        waited = true;
+#pragma unroll 1
+        for (int t = t0; t < tokens; t += together) {
+            Unit<X, L> units[kItems];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int x = x0 + k * step;
-            if (x >= total) break;
-            const int hh = div_by(x, p.by_units), t = div_by(hh, p.by_heads), head = hh - t * p.heads, u = x - hh * p.units;
-            const long long i = first + t, slot = slots[t];
-            const int kvh = head - p.q_heads;
-            if (kvh < 0) {
-                X* dst = static_cast<X*>(a.q_out) + i * a.out_token_stride + head * a.out_head_stride;
-                write_unit<X, X, WIDE>(p, u, true, slot == -2, units[k], dst, cos[t], sin[t]);
-            } else if (slot >= 0) {
-                const bool is_v = kvh >= p.pg.n_kv_heads;
-                KV* dst = static_cast<KV*>(is_v ? p.pg.v : p.pg.k) + slot + (is_v ? kvh - p.pg.n_kv_heads : kvh) * p.pg.head_stride;
-                write_unit<X, KV, WIDE>(p, u, !is_v, false, units[k], dst, cos[t], sin[t]);
+            for (int j = 0; j < kItems; ++j) {
+                if (src[j] == nullptr) break;
+                units[j].load(w, src[j]);
+                src[j] += ahead[j];
+            }
+            const long long slot = slots[t];
+#pragma unroll
+            for (int j = 0; j < Job<L>::kPairs; ++j) {
+                w.c[j] = w.pair ? cos[t][u * Job<L>::kPairs + j] : 0.f;
+                w.s[j] = w.pair ? sin[t][u * Job<L>::kPairs + j] : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < kItems; ++j) {
+                if (src[j] == nullptr) break;
+                if (out[j] != nullptr) {
+                    if (slot == -2) units[j].clear();
+                    units[j].store(w, true, out[j]);
+                    out[j] += together * a.out_token_stride;
+                } else if (slot >= 0) {
+                    units[j].store(w, rotates[j], page[j] + slot);
+                }
             }
         }
     }
@@ -207,15 +284,18 @@ void launch_for(Params& p, cudaStream_t stream) {
     const int dims = wide ? 8 : 1;
     p.pair_units = wide && a.interleaved ? a.rotary / 8 : p.pairs / dims;
     p.units = p.pair_units + (p.pg.head_dim - a.rotary) / dims;
-    p.by_units = fast_div(p.units);
-    p.by_heads = fast_div(p.heads);
-    // Blocks of about three units a thread; where that leaves SMs idle, one token and its heads spread over several blocks.
+    // Up to 8 tokens a block, since what a block sets up once costs as much as a dozen units of a thread; with fewer blocks than
+    // fill the GPU four deep, fewer tokens; and with less than one token for each SM, a token's heads on several blocks.
     const int token_units = p.units * p.heads, sms = num_sms();
-    p.tokens = std::max(1, std::min(kTokens, kBatch * kThreads / token_units));
-    if (a.n_tokens / p.tokens < 2 * sms) p.tokens = std::max(1, std::min(p.tokens, a.n_tokens / (2 * sms)));
+    p.tokens = std::max(1, std::min(kTokens, a.n_tokens / (4 * sms)));
+    const int small = std::max(1, std::min(kTokens, kThreads / token_units));  // tokens that keep a block's threads busy
+    if (p.tokens < small && a.n_tokens / small >= sms) p.tokens = small;
     const int blocks = (a.n_tokens + p.tokens - 1) / p.tokens;
     const int spread = blocks >= 2 * sms ? 1 : std::max(1, std::min((p.tokens * token_units + kThreads - 1) / kThreads, 2 * sms / blocks));
-    launch_kernel(wide ? append_kernel<X, KV, true> : append_kernel<X, KV, false>, dim3(blocks, spread), dim3(kThreads), 0, stream, false, p);
+    auto kernel = !wide           ? append_kernel<X, KV, Layout::kSingle>
+                  : a.interleaved ? append_kernel<X, KV, Layout::kInterleaved>
+                                  : append_kernel<X, KV, Layout::kHalves>;
+    launch_kernel(kernel, dim3(blocks, spread), dim3(kThreads), 0, stream, false, p);
 }
 
 template <typename X>

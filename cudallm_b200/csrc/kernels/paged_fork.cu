@@ -1,19 +1,29 @@
 // Bookkeeping of a paged cache's sequences: forking (sharing, copy on write, freeing, new pages) and compaction.
 //
-// Both run as a plan kernel of one block, which decides who gets which page (all of it integer prefix sums, so the
-// result does not depend on any order of threads), and a kernel over the whole GPU that moves the tokens of every
-// layer and writes tables and references.
+// Both run as a plan kernel, whose first block decides who gets which page (all of it integer prefix sums, so the result
+// does not depend on any order of threads), and a kernel over the whole GPU, in place when the plan is done, that moves
+// the tokens of every layer and writes tables and references. The moves read and write each byte once and HBM bounds
+// them; with few of them the plan's chain of dependent loads (parent, length, entry, references) does.
+#include <algorithm>
 #include <climits>
 
 #include "common/check.h"
+#include "kernels/kernels.h"
+#include "kernels/launch.cuh"
 #include "kernels/paged.h"
+#include "kernels/paged_common.cuh"
+#include "kernels/ptx.cuh"
 
 namespace cudallm {
 
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kEach = 16;  // pages of a thread in one pass over the references
+constexpr int kPass = kPlanThreads * kEach;
 constexpr int kMoveThreads = 256;
+constexpr int kSharedRows = 4096;  // rows whose counters fit the plan's shared memory
+constexpr unsigned kAll = 0xffffffffu;
 
 // Exclusive prefix sum of one value per thread over the block; `total` gets the sum. Barriers on both sides.
 __device__ int block_scan(int v, int* sm, int& total) {
@@ -21,69 +31,133 @@ __device__ int block_scan(int v, int* sm, int& total) {
     int s = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, s, o);
+        const int t = __shfl_up_sync(kAll, s, o);
         if (lane >= o) s += t;
     }
     __syncthreads();
     if (lane == 31) sm[warp] = s;
     __syncthreads();
-    if (warp == 0) {
-        int w = sm[lane];
+    int w = sm[lane];  // every warp sums the warps' totals for itself
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += t;
-        }
-        sm[lane] = w;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(kAll, w, o);
+        if (lane >= o) w += t;
     }
-    __syncthreads();
-    total = sm[31];
-    return s - v + (warp > 0 ? sm[warp - 1] : 0);
-}
-
-// Scratch of a fork: per parent row the number of children, the first child, the entries held and whether the pages
-// from the first not full one on are its own; per new row the first rank among the new pages; the new pages by rank.
-struct ForkScratch {
-    int *children, *first, *held, *alone, *start, *fresh, *found;
-    int* n_found;
-};
-
-__host__ __device__ inline ForkScratch fork_scratch(void* workspace, int rows) {
-    int* p = static_cast<int*>(workspace);
-    ForkScratch s;
-    s.n_found = p;
-    p += 64;
-    s.children = p;
-    s.first = p + rows;
-    s.held = p + 2 * rows;
-    s.alone = p + 3 * rows;
-    s.start = p + 4 * rows;
-    s.fresh = p + 5 * rows;
-    s.found = p + 6 * rows;
-    return s;
+    total = __shfl_sync(kAll, w, 31);
+    const int before = __shfl_sync(kAll, w, (warp + 31) & 31);
+    return s - v + (warp > 0 ? before : 0);
 }
 
 __device__ __forceinline__ bool is_page(int p, int n_pages) { return p >= 0 && p < n_pages; }
+
+// This thread's kEach references from p on (p a multiple of kEach); pages past the end read as `none`.
+__device__ __forceinline__ void load_refs(const int* refs, int p, int n, int none, bool wide, int (&r)[kEach]) {
+    if (wide && p + kEach <= n) {
+#pragma unroll
+        for (int i = 0; i < kEach; i += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(refs + p + i);
+            r[i] = v.x, r[i + 1] = v.y, r[i + 2] = v.z, r[i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) r[i] = p + i < n ? refs[p + i] : none;
+    }
+}
+
+// One warp copies `tokens` tokens of one head of one page of one layer, of k and of v.
+__device__ __forceinline__ void copy_head(const cudallm_pages& pg, FastDiv by_row, int layer, int head, int src, int dst, int tokens) {
+    const int per_row = pg.head_dim / 8, n = tokens * per_row, lane = threadIdx.x & 31;  // 16-byte words
+    const long long base = layer * pg.layer_stride + head * pg.head_stride;
+    const uint16_t *ks = static_cast<const uint16_t*>(pg.k) + base + src * pg.page_stride, *vs = static_cast<const uint16_t*>(pg.v) + base + src * pg.page_stride;
+    uint16_t *kd = static_cast<uint16_t*>(pg.k) + base + dst * pg.page_stride, *vd = static_cast<uint16_t*>(pg.v) + base + dst * pg.page_stride;
+    constexpr int kAtOnce = 4;
+    for (int c0 = lane; c0 < n; c0 += 32 * kAtOnce) {
+        uint4 k[kAtOnce], v[kAtOnce];
+        long long at[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int c = c0 + 32 * i;
+            if (c >= n) break;
+            const int t = div_by(c, by_row);
+            at[i] = t * pg.token_stride + (c - t * per_row) * 8;
+            k[i] = *reinterpret_cast<const uint4*>(ks + at[i]);
+            v[i] = *reinterpret_cast<const uint4*>(vs + at[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (c0 + 32 * i >= n) break;
+            *reinterpret_cast<uint4*>(kd + at[i]) = k[i];
+            *reinterpret_cast<uint4*>(vd + at[i]) = v[i];
+        }
+    }
+}
+
+// ---- fork ----------------------------------------------------------------------------------------
+
+struct OutRow {
+    int parent, len, from, start;  // the parent (-1: empty), its length, its entries that are taken over, rank of the first new page
+};
+struct OldRow {
+    int full, held, children, kept;  // full pages, entries held, children, whether a child takes over what follows the full pages
+};
+struct Copy {
+    int src, dst, tokens, pad;
+};
+struct ForkPlan {
+    int* totals;  // new pages found, copies
+    OutRow* out;
+    OldRow* old;
+    Copy* copies;
+    int *fresh, *children, *first, *found;
+};
+
+// Bytes of a plan for that many rows, and its parts in a workspace.
+__host__ __device__ inline size_t fork_plan_bytes(int n_pages, int rows) { return 256 + (3 * 16 + 3 * 4) * static_cast<size_t>(rows) + 4 * static_cast<size_t>(n_pages); }
+inline ForkPlan fork_plan(void* workspace, int rows) {
+    char* p = static_cast<char*>(workspace);
+    ForkPlan s;
+    s.totals = reinterpret_cast<int*>(p);
+    s.out = reinterpret_cast<OutRow*>(p + 256);
+    s.old = reinterpret_cast<OldRow*>(s.out + rows);
+    s.copies = reinterpret_cast<Copy*>(s.old + rows);
+    s.fresh = reinterpret_cast<int*>(s.copies + rows);
+    s.children = s.fresh + rows;
+    s.first = s.children + rows;
+    s.found = s.first + rows;
+    return s;
+}
 
 __device__ __forceinline__ int row_len(const cudallm_pages& pg, const cudallm_fork_args& a, int r) {
     const long long cap = static_cast<long long>(a.table_width) * pg.page_size;
     return static_cast<int>(min(static_cast<long long>(max(a.lens[r], 0)), cap));
 }
 
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(cudallm_pages pg, cudallm_fork_args a, ForkScratch s) {
+// Block 0 plans; the others copy the references, which the move kernel then changes.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
+                                                                 bool wide) {
+    extern __shared__ int counters[];  // children and first child of up to kSharedRows rows
     __shared__ int sm[32];
-    __shared__ unsigned long long sm_over;
-    for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {
-        s.children[r] = 0;
-        s.first[r] = INT_MAX;
+    __shared__ unsigned long long over;
+    grid_dep_launch();
+    if (blockIdx.x > 0) {
+        for (int p = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; p < pg.n_pages; p += (gridDim.x - 1) * kPlanThreads) a.refs_out[p] = a.refs[p];
+        return;
     }
-    if (threadIdx.x == 0) sm_over = 0;
+    int refs[kEach];  // of the first pass, under way while the rows are looked at
+    load_refs(a.refs, threadIdx.x * kEach, pg.n_pages, 1, wide, refs);
+    int* children = a.n_rows <= kSharedRows ? counters : s.children;
+    int* first = a.n_rows <= kSharedRows ? counters + a.n_rows : s.first;
+    for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {
+        children[r] = 0;
+        first[r] = INT_MAX;
+    }
+    if (threadIdx.x == 0) over = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < a.n_out; i += kPlanThreads) {
         const int p = a.parents[i];
         if (p >= 0 && p < a.n_rows) {
-            atomicAdd(&s.children[p], 1);
-            atomicMin(&s.first[p], i);
+            atomicAdd(&children[p], 1);
+            atomicMin(&first[p], i);
         }
     }
     for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {
@@ -91,199 +165,228 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(cudallm_pages p
         const int* row = a.tables + r * a.table_stride;
         int held = full;
         while (held < a.table_width && is_page(row[held], pg.n_pages)) ++held;
-        s.held[r] = held;
-        s.alone[r] = held > full && a.refs[row[full]] == 1;
+        s.old[r] = {full, held, 0, held > full && a.refs[row[full]] == 1};
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {  // a thread's own rows
+        s.old[r].children = children[r];
+        if (children[r] == 0) s.old[r].kept = 0;
     }
     __syncthreads();
     int base = 0;
     for (int i0 = 0; i0 < a.n_out; i0 += kPlanThreads) {
         const int i = i0 + threadIdx.x;
         int fresh = 0;
+        OutRow o{-1, 0, 0, 0};
         if (i < a.n_out) {
             const int p = a.parents[i];
             if (p >= 0 && p < a.n_rows) {
-                const long long len = row_len(pg, a, p);
-                const long long want = (len + a.room + pg.page_size - 1) / pg.page_size;
-                const bool keeps = s.alone[p] && s.first[p] == i;
-                const int from = keeps ? s.held[p] : static_cast<int>(len / pg.page_size);
-                fresh = static_cast<int>(max(0LL, min(want, static_cast<long long>(a.table_width)) - from));
-                if (want > a.table_width) atomicAdd(&sm_over, static_cast<unsigned long long>(want - a.table_width));
+                const OldRow old = s.old[p];
+                o.parent = p;
+                o.len = row_len(pg, a, p);
+                o.from = old.kept && first[p] == i ? old.held : old.full;
+                const long long want = (static_cast<long long>(o.len) + a.room + pg.page_size - 1) / pg.page_size;
+                fresh = static_cast<int>(max(0LL, min(want, static_cast<long long>(a.table_width)) - o.from));
+                if (want > a.table_width) atomicAdd(&over, static_cast<unsigned long long>(want - a.table_width));
             }
         }
         int total;
-        const int at = block_scan(fresh, sm, total);
+        o.start = base + block_scan(fresh, sm, total);
         if (i < a.n_out) {
-            s.start[i] = base + at;
+            s.out[i] = o;
             s.fresh[i] = fresh;
         }
         base += total;
     }
     int found = 0;
-    for (int p0 = 0; p0 < pg.n_pages && found < base; p0 += kPlanThreads) {
-        const int p = p0 + threadIdx.x;
-        const int free = p < pg.n_pages && a.refs[p] == 0;
-        int total;
-        const int at = block_scan(free, sm, total);
-        if (free && found + at < base) s.found[found + at] = p;
+    for (int p0 = 0; p0 < pg.n_pages && found < base; p0 += kPass) {
+        const int p = p0 + threadIdx.x * kEach;
+        if (p0 > 0) load_refs(a.refs, p, pg.n_pages, 1, wide, refs);
+        int n = 0, total;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n += refs[i] == 0;
+        int at = found + block_scan(n, sm, total);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (refs[i] == 0 && at < base) s.found[at] = p + i;
+            at += refs[i] == 0;
+        }
         found += total;
     }
+    found = min(found, base);
     __syncthreads();
+    int copies = 0;
+    for (int i0 = 0; i0 < a.n_out; i0 += kPlanThreads) {
+        const int i = i0 + threadIdx.x;
+        Copy c{0, 0, 0, 0};
+        if (i < a.n_out) {
+            const OutRow o = s.out[i];
+            if (o.parent >= 0) {
+                const OldRow old = s.old[o.parent];
+                const int tail = o.len - old.full * pg.page_size;
+                const bool keeps = old.kept && first[o.parent] == i;
+                if (!keeps && tail > 0 && old.held > old.full && s.fresh[i] > 0 && o.start < found) {
+                    c = {a.tables[o.parent * a.table_stride + old.full], s.found[o.start], tail, 0};
+                }
+            }
+        }
+        int total;
+        const int at = copies + block_scan(c.tokens > 0, sm, total);
+        if (c.tokens > 0) s.copies[at] = c;
+        copies += total;
+    }
     if (threadIdx.x == 0) {
-        found = min(found, base);
-        *s.n_found = found;
-        const unsigned long long missing = sm_over + static_cast<unsigned long long>(base - found);
+        s.totals[0] = found;
+        s.totals[1] = copies;
+        const unsigned long long missing = over + static_cast<unsigned long long>(base - found);
         *a.missing = static_cast<int>(min(missing, static_cast<unsigned long long>(INT_MAX)));
     }
 }
 
-// Copies `tokens` tokens of one page of one layer, all heads, of k and v.
-template <typename Vec>
-__device__ void copy_page(const cudallm_pages& pg, int layer, int src, int dst, int tokens) {
-    constexpr int kElems = sizeof(Vec) / 2;
-    const int per_row = pg.head_dim / kElems;
-    const int total = tokens * pg.n_kv_heads * per_row;
-    const long long l = layer * pg.layer_stride;
-    for (int u = threadIdx.x; u < total; u += blockDim.x) {
-        const int c = u % per_row, t = u / per_row % tokens, h = u / per_row / tokens;
-        const long long at = l + h * pg.head_stride + t * pg.token_stride + c * kElems;
-        const long long from = at + src * pg.page_stride, to = at + dst * pg.page_stride;
-        *reinterpret_cast<Vec*>(static_cast<uint16_t*>(pg.k) + to) = *reinterpret_cast<const Vec*>(static_cast<const uint16_t*>(pg.k) + from);
-        *reinterpret_cast<Vec*>(static_cast<uint16_t*>(pg.v) + to) = *reinterpret_cast<const Vec*>(static_cast<const uint16_t*>(pg.v) + from);
-    }
-}
-
-// Block (i, y): y == 0 writes row i of the outputs and, for parent row i, the references its pages lose or gain;
-// the blocks of a row share its copy's layers.
-__global__ void __launch_bounds__(kMoveThreads) fork_move_kernel(cudallm_pages pg, cudallm_fork_args a, ForkScratch s) {
+// The first `rows` blocks: row i of the outputs, and the references that parent row i's pages lose or gain. The other blocks' warps
+// each copy heads of pages.
+__global__ void __launch_bounds__(kMoveThreads) fork_move_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
+                                                                 int rows, FastDiv by_row) {
+    grid_dep_wait();
     const int i = blockIdx.x;
-    const int n_found = *s.n_found;
-    if (blockIdx.y == 0 && i < a.n_rows) {
-        const int full = row_len(pg, a, i) / pg.page_size, held = s.held[i], kids = s.children[i];
-        const bool kept = s.alone[i] && kids > 0;
-        for (int j = threadIdx.x; j < held; j += kMoveThreads) {
+    if (i >= rows) {
+        const long long units = static_cast<long long>(s.totals[1]) * pg.n_layers * pg.n_kv_heads;
+        const long long step = static_cast<long long>(gridDim.x - rows) * (kMoveThreads / 32);
+        for (long long u = static_cast<long long>(i - rows) * (kMoveThreads / 32) + threadIdx.x / 32; u < units; u += step) {
+            const int head = static_cast<int>(u % pg.n_kv_heads), layer = static_cast<int>(u / pg.n_kv_heads % pg.n_layers);
+            const Copy c = s.copies[u / pg.n_kv_heads / pg.n_layers];
+            copy_head(pg, by_row, layer, head, c.src, c.dst, c.tokens);
+        }
+        return;
+    }
+    if (i < a.n_rows) {
+        const OldRow old = s.old[i];
+        for (int j = threadIdx.x; j < old.held; j += kMoveThreads) {
             const int p = a.tables[i * a.table_stride + j];
-            const int gain = j < full ? kids - 1 : kept ? 0 : -1;
+            const int gain = j < old.full ? old.children - 1 : old.kept ? 0 : -1;
             if (gain != 0 && is_page(p, pg.n_pages)) atomicAdd(&a.refs_out[p], gain);
         }
     }
     if (i >= a.n_out) return;
-    const int parent = a.parents[i];
-    const bool alive = parent >= 0 && parent < a.n_rows;
-    const int len = alive ? row_len(pg, a, parent) : 0, full = len / pg.page_size;
-    const bool keeps = alive && s.alone[parent] && s.first[parent] == i;
-    const int from = keeps ? s.held[parent] : full, start = s.start[i], fresh = s.fresh[i];
-    const int* old = a.tables + static_cast<long long>(alive ? parent : 0) * a.table_stride;
-    if (blockIdx.y == 0) {
-        for (int j = threadIdx.x; j < a.table_width; j += kMoveThreads) {
-            int e = -1;
-            if (alive && j < from) {
-                e = is_page(old[j], pg.n_pages) ? old[j] : -1;
-            } else if (alive && j < from + fresh && start + j - from < n_found) {
-                e = s.found[start + j - from];
-                atomicAdd(&a.refs_out[e], 1);
-            }
-            a.tables_out[i * a.table_out_stride + j] = e;
+    const OutRow o = s.out[i];
+    const int n_found = s.totals[0], fresh = s.fresh[i];
+    const int* old = a.tables + static_cast<long long>(max(o.parent, 0)) * a.table_stride;
+    for (int j = threadIdx.x; j < a.table_width; j += kMoveThreads) {
+        int e = -1;
+        if (o.parent >= 0 && j < o.from) {
+            e = is_page(old[j], pg.n_pages) ? old[j] : -1;
+        } else if (j < o.from + fresh && o.start + j - o.from < n_found) {
+            e = s.found[o.start + j - o.from];
+            atomicAdd(&a.refs_out[e], 1);
         }
-        if (threadIdx.x == 0) a.lens_out[i] = len;
+        a.tables_out[i * a.table_out_stride + j] = e;
     }
-    const int tail = len - full * pg.page_size;
-    if (alive && !keeps && tail > 0 && s.held[parent] > full && fresh > 0 && start < n_found) {
-        for (int l = blockIdx.y; l < pg.n_layers; l += gridDim.y) copy_page<uint4>(pg, l, old[full], s.found[start], tail);
-    }
+    if (threadIdx.x == 0) a.lens_out[i] = o.len;
 }
 
-struct CompactScratch {
-    int *to, *src, *dst;
-    int* n_moves;
+// ---- compact ---------------------------------------------------------------------------------------
+
+struct CompactPlan {
+    int* totals;          // pages in use, moves
+    int *to, *src, *dst;  // new place of a page that moves; the moves
 };
-
-__host__ __device__ inline CompactScratch compact_scratch(void* workspace, int n_pages) {
+inline CompactPlan compact_plan(void* workspace, int n_pages) {
     int* p = static_cast<int*>(workspace);
-    CompactScratch s;
-    s.n_moves = p;
-    p += 64;
-    s.to = p;
-    s.src = p + n_pages;
-    s.dst = p + 2 * static_cast<size_t>(n_pages);
-    return s;
+    return {p, p + 64, p + 64 + n_pages, p + 64 + 2 * static_cast<size_t>(n_pages)};
 }
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(cudallm_pages pg, cudallm_compact_args a, CompactScratch s) {
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
+                                                                    bool wide) {
     __shared__ int sm[32];
-    int live = 0;
-    for (int p0 = 0; p0 < pg.n_pages; p0 += kPlanThreads) {
-        const int p = p0 + threadIdx.x;
-        int total;
-        block_scan(p < pg.n_pages && a.refs[p] > 0, sm, total);
+    grid_dep_launch();
+    int refs[kEach], live = 0;
+    for (int p0 = 0; p0 < pg.n_pages; p0 += kPass) {
+        load_refs(a.refs, p0 + threadIdx.x * kEach, pg.n_pages, 0, wide, refs);
+        int n = 0, total;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n += refs[i] > 0;
+        block_scan(n, sm, total);
         live += total;
     }
     int holes = 0, movers = 0;
-    for (int p0 = 0; p0 < pg.n_pages; p0 += kPlanThreads) {
-        const int p = p0 + threadIdx.x;
-        const bool in = p < pg.n_pages, used = in && a.refs[p] > 0;
-        const bool hole = in && !used && p < live, mover = used && p >= live;
-        int total;
-        const int h = block_scan(hole, sm, total) + holes;
-        holes += total;
-        const int m = block_scan(mover, sm, total) + movers;
-        movers += total;
-        if (hole) s.dst[h] = p;
-        if (mover) s.src[m] = p;
-        if (in) {
-            s.to[p] = p;
-            a.refs_out[p] = used && p < live ? a.refs[p] : 0;
+    for (int p0 = 0; p0 < pg.n_pages; p0 += kPass) {
+        const int p = p0 + threadIdx.x * kEach;
+        if (pg.n_pages > kPass) load_refs(a.refs, p, pg.n_pages, 0, wide, refs);
+        int n = 0, total;  // holes in the low half, movers in the high one: a pass has at most 16384 of each
+        static_assert(kPass < 1 << 15, "two counts in one int");
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n += refs[i] > 0 ? (p + i >= live) << 16 : p + i < live;
+        const int at = block_scan(n, sm, total);
+        int h = holes + (at & 0xffff), m = movers + (at >> 16);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (refs[i] > 0 && p + i >= live) s.src[m++] = p + i;
+            if (refs[i] <= 0 && p + i < live) s.dst[h++] = p + i;
         }
+        holes += total & 0xffff;
+        movers += total >> 16;
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < movers; k += kPlanThreads) {
-        s.to[s.src[k]] = s.dst[k];
-        a.refs_out[s.dst[k]] = a.refs[s.src[k]];
-    }
+    for (int k = threadIdx.x; k < movers; k += kPlanThreads) s.to[s.src[k]] = s.dst[k];
     if (threadIdx.x == 0) {
-        *s.n_moves = movers;
+        s.totals[0] = live;
+        s.totals[1] = movers;
         *a.live = live;
     }
 }
 
-__global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(cudallm_pages pg, cudallm_compact_args a, CompactScratch s) {
-    const long long moves = static_cast<long long>(*s.n_moves) * pg.n_layers;
-    for (long long u = blockIdx.x; u < moves; u += gridDim.x) {
-        copy_page<uint4>(pg, static_cast<int>(u % pg.n_layers), s.src[u / pg.n_layers], s.dst[u / pg.n_layers], pg.page_size);
+__global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
+                                                                    FastDiv by_row) {
+    grid_dep_wait();
+    const int live = s.totals[0];
+    const long long threads = static_cast<long long>(gridDim.x) * kMoveThreads, me = static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x;
+    for (long long p = me; p < pg.n_pages; p += threads) {
+        const int r = a.refs[p];
+        if (p >= live) a.refs_out[p] = 0;
+        if (r > 0) a.refs_out[p < live ? p : s.to[p]] = r;
     }
     const long long entries = static_cast<long long>(a.n_rows) * a.table_width;
-    for (long long e = static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x; e < entries;
-         e += static_cast<long long>(gridDim.x) * kMoveThreads) {
+    for (long long e = me; e < entries; e += threads) {
         const long long r = e / a.table_width, j = e % a.table_width;
         const int p = a.tables[r * a.table_stride + j];
-        a.tables_out[r * a.table_out_stride + j] = is_page(p, pg.n_pages) ? s.to[p] : -1;
+        a.tables_out[r * a.table_out_stride + j] = !is_page(p, pg.n_pages) ? -1 : p >= live && a.refs[p] > 0 ? s.to[p] : p;
+    }
+    const long long units = static_cast<long long>(s.totals[1]) * pg.n_layers * pg.n_kv_heads;
+    for (long long u = me / 32; u < units; u += threads / 32) {
+        const int head = static_cast<int>(u % pg.n_kv_heads), layer = static_cast<int>(u / pg.n_kv_heads % pg.n_layers);
+        const int k = static_cast<int>(u / pg.n_kv_heads / pg.n_layers);
+        copy_head(pg, by_row, layer, head, s.src[k], s.dst[k], pg.page_size);
     }
 }
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 
 size_t pages_workspace_bytes(int n_pages, int rows) {
     if (n_pages < 1 || rows < 0 || rows > kMaxPageRows) return 0;
-    const size_t fork = 6 * static_cast<size_t>(rows) + n_pages, compact = 3 * static_cast<size_t>(n_pages);
-    return 4 * (64 + (fork > compact ? fork : compact));
+    return std::max(fork_plan_bytes(n_pages, rows), 256 + 12 * static_cast<size_t>(n_pages));
 }
 
 void launch_paged_fork(const cudallm_pages& pg, const cudallm_fork_args& a, cudaStream_t stream) {
-    const int rows = a.n_rows > a.n_out ? a.n_rows : a.n_out;
-    CLLM_CUDA(cudaMemcpyAsync(a.refs_out, a.refs, sizeof(int) * static_cast<size_t>(pg.n_pages), cudaMemcpyDeviceToDevice, stream));
-    const ForkScratch s = fork_scratch(a.workspace, rows);
-    fork_plan_kernel<<<1, kPlanThreads, 0, stream>>>(pg, a, s);
-    CLLM_CUDA(cudaGetLastError());
+    const int rows = std::max(a.n_rows, a.n_out), sms = num_sms();
+    const ForkPlan s = fork_plan(a.workspace, rows);
+    const int copiers = std::min(sms, (pg.n_pages + kPlanThreads - 1) / kPlanThreads);  // of the references
+    const size_t smem = a.n_rows <= kSharedRows ? 8 * static_cast<size_t>(a.n_rows) : 0;
+    launch_kernel(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), smem, stream, false, pg, a, s, aligned16(a.refs));
     if (rows == 0) return;
-    fork_move_kernel<<<dim3(rows, pg.n_layers < 64 ? pg.n_layers : 64), kMoveThreads, 0, stream>>>(pg, a, s);
-    CLLM_CUDA(cudaGetLastError());
+    const long long heads = static_cast<long long>(a.n_out) * pg.n_layers * pg.n_kv_heads;
+    const int movers = static_cast<int>(std::min<long long>(8LL * sms, (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
+    launch_kernel(fork_move_kernel, dim3(rows + movers), dim3(kMoveThreads), 0, stream, true, pg, a, s, rows, fast_div(pg.head_dim / 8));
 }
 
 void launch_paged_compact(const cudallm_pages& pg, const cudallm_compact_args& a, cudaStream_t stream) {
-    const CompactScratch s = compact_scratch(a.workspace, pg.n_pages);
-    compact_plan_kernel<<<1, kPlanThreads, 0, stream>>>(pg, a, s);
-    CLLM_CUDA(cudaGetLastError());
-    compact_move_kernel<<<8 * 148, kMoveThreads, 0, stream>>>(pg, a, s);
-    CLLM_CUDA(cudaGetLastError());
+    const CompactPlan s = compact_plan(a.workspace, pg.n_pages);
+    launch_kernel(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, false, pg, a, s, aligned16(a.refs));
+    // No page moves onto another that stays, so at most half of the pages move.
+    const long long heads = static_cast<long long>(pg.n_pages / 2) * pg.n_layers * pg.n_kv_heads;
+    const int blocks = static_cast<int>(std::min<long long>(8LL * num_sms(), 1 + (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
+    launch_kernel(compact_move_kernel, dim3(blocks), dim3(kMoveThreads), 0, stream, true, pg, a, s, fast_div(pg.head_dim / 8));
 }
 
 }  // namespace cudallm

@@ -18,6 +18,7 @@ include/cudallm.h states. A cache serves one host thread at a time.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import threading
 
@@ -56,6 +57,11 @@ def _args(name: str):
 
 
 _beam = threading.local()
+
+
+@functools.cache
+def _beam_calls():
+    return lib().cudallm_beam_select, lib().cudallm_beam_workspace_bytes
 
 
 def _beam_args():
@@ -103,30 +109,30 @@ class _OnDevice:
 
 
 def _int32(t: torch.Tensor, device: torch.device, shape: tuple, name: str) -> int:
-    if t.dtype is not torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != device.index or t.shape != shape or not t.is_contiguous():
         _refuse(f"{name} must be a contiguous int32 tensor {list(shape)} on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
 def _table(t: torch.Tensor, device: torch.device, name: str) -> tuple[int, int, int]:
     """(rows, width, row stride) of a page table."""
-    if t.dtype is not torch.int32 or t.device != device or t.dim() != 2:
+    if t.dtype is not torch.int32 or t.get_device() != device.index or t.dim() != 2:
         _refuse(f"{name} must be an int32 tensor [rows][width] on {device}")
     rows, width = t.shape
     stride, inner = t.stride()
-    if rows and width > 1 and inner != 1:
+    if inner != 1 and rows and width > 1:
         _refuse(f"{name} must have its entries side by side")
     return rows, width, stride
 
 
 def _heads(t: torch.Tensor, device: torch.device, dtype: torch.dtype, dim: int, name: str) -> tuple[int, int, int, int]:
     """(tokens, heads, token stride, head stride) of [tokens][heads][dim]."""
-    if t.dtype is not dtype or t.device != device or t.dim() != 3 or t.shape[2] != dim:
+    if t.dtype is not dtype or t.get_device() != device.index or t.dim() != 3:
         _refuse(f"{name} must be a {dtype} tensor [tokens][heads][{dim}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
-    n, heads, _ = t.shape
+    n, heads, d = t.shape
     ts, hs, inner = t.stride()
-    if inner != 1 and n and heads:
-        _refuse(f"{name} must have its dims side by side")
+    if d != dim or (inner != 1 and n and heads):
+        _refuse(f"{name} must be [tokens][heads][{dim}] with its dims side by side, got {list(t.shape)} with strides {list(t.stride())}")
     return n, heads, ts, hs
 
 
@@ -187,6 +193,8 @@ class PagedCache:
         self._fork, self._fork_ref = _args("cudallm_fork_args")
         self._compact, self._compact_ref = _args("cudallm_compact_args")
         self._workspaces = _Workspaces(self.device)
+        self._scale = self.head_dim ** -0.5
+        self._pages_bytes: dict[int, int] = {}  # workspace of fork and compact by rows
         self._attend_bytes = self._lib.cudallm_attend_workspace_bytes()
         check(self._lib.cudallm_paged_attend(self._pages, self._attend_ref, None))  # no rows: checks the pool alone
 
@@ -215,6 +223,12 @@ class PagedCache:
         a.workspace, a.workspace_bytes = w.data_ptr(), w.numel()
         return w
 
+    def _pages_size(self, rows: int) -> int:
+        size = self._pages_bytes.get(rows)
+        if size is None:
+            size = self._pages_bytes[rows] = self._lib.cudallm_pages_workspace_bytes(self.n_pages, rows)
+        return size
+
     def attend(self, q: torch.Tensor, tables: torch.Tensor, lens: torch.Tensor, *, layer: int = 0, scale: float | None = None,
                window: int = 0, out: torch.Tensor | None = None, with_lse: bool = False):
         """Attention of one new token per row: q [rows][heads][head dim] (fp32, fp16 or bf16) over the first lens[row] tokens of
@@ -235,7 +249,7 @@ class PagedCache:
             _refuse("out must be contiguous, with q's shape and type")
         lse = q.new_empty((n, heads), dtype=torch.float32) if with_lse else None
         a.layer, a.x_dtype, a.n_seq, a.n_heads, a.table_width, a.window = layer, x, n, heads, width, window
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        a.scale = self._scale if scale is None else scale
         a.q, a.q_seq_stride, a.q_head_stride = q.data_ptr(), a_seq, a_head
         a.tables, a.table_stride, a.out = tables.data_ptr(), stride, out.data_ptr()
         a.lse = None if lse is None else lse.data_ptr()
@@ -266,9 +280,11 @@ class PagedCache:
                 _refuse("q, k and v must have the same number of tokens")
             if out is None:
                 out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                a.out_token_stride, a.out_head_stride = heads * dim, dim
             elif out.shape != q.shape:
                 _refuse("out must have q's shape")
-            _, _, a.out_token_stride, a.out_head_stride = _heads(out, dev, k.dtype, dim, "out")
+            else:
+                _, _, a.out_token_stride, a.out_head_stride = _heads(out, dev, k.dtype, dim, "out")
             a.q, a.q_out = q.data_ptr(), out.data_ptr()
         elif out is not None:
             _refuse("out needs a q")
@@ -293,22 +309,28 @@ class PagedCache:
         `out` = such a tuple to write, which must not overlap the inputs (a program keeps two and swaps them)."""
         dev, a = self.device, self._fork
         n_rows, width, a.table_stride = _table(tables, dev, "tables")
-        n_out = parents.shape[0] if parents.dim() == 1 else _refuse("parents must be a vector")
+        if parents.dim() != 1:
+            _refuse("parents must be a vector")
+        n_out = parents.shape[0]
         a.lens = _int32(lens, dev, (n_rows,), "lens")
         a.refs = _int32(refs, dev, (self.n_pages,), "refs")
         a.parents = _int32(parents, dev, (n_out,), "parents")
+        a.tables = tables.data_ptr()
         if out is None:
-            out = (tables.new_empty((n_out, width)), torch.empty_like(parents), torch.empty_like(refs), refs.new_empty(1))
-        t_rows, t_width, a.table_out_stride = _table(out[0], dev, "out tables")
-        if t_rows != n_out or t_width != width:
-            _refuse(f"out tables must be [{n_out}][{width}]")
-        a.lens_out = _int32(out[1], dev, (n_out,), "out lens")
-        a.refs_out = _int32(out[2], dev, (self.n_pages,), "out refs")
-        a.missing = _int32(out[3], dev, (1,), "missing")
+            out = t, n, r, missing = tables.new_empty((n_out, width)), torch.empty_like(parents), torch.empty_like(refs), refs.new_empty(1)
+            a.tables_out, a.table_out_stride = t.data_ptr(), width
+            a.lens_out, a.refs_out, a.missing = n.data_ptr(), r.data_ptr(), missing.data_ptr()
+        else:
+            t_rows, t_width, a.table_out_stride = _table(out[0], dev, "out tables")
+            if t_rows != n_out or t_width != width:
+                _refuse(f"out tables must be [{n_out}][{width}]")
+            a.tables_out = out[0].data_ptr()
+            a.lens_out = _int32(out[1], dev, (n_out,), "out lens")
+            a.refs_out = _int32(out[2], dev, (self.n_pages,), "out refs")
+            a.missing = _int32(out[3], dev, (1,), "missing")
         a.n_rows, a.n_out, a.table_width, a.room = n_rows, n_out, width, room
-        a.tables, a.tables_out = tables.data_ptr(), out[0].data_ptr()
         stream = _stream_of(self._index)
-        keep = self._workspace(a, self._lib.cudallm_pages_workspace_bytes(self.n_pages, max(n_rows, n_out)), stream)  # noqa: F841
+        keep = self._workspace(a, self._pages_size(n_rows if n_rows > n_out else n_out), stream)  # noqa: F841
         self._run(self._call_fork, self._fork_ref, stream)
         return out
 
@@ -318,17 +340,20 @@ class PagedCache:
         dev, a = self.device, self._compact
         n_rows, width, a.table_stride = _table(tables, dev, "tables")
         a.refs = _int32(refs, dev, (self.n_pages,), "refs")
+        a.tables = tables.data_ptr()
         if out is None:
-            out = (tables.new_empty((n_rows, width)), torch.empty_like(refs), refs.new_empty(1))
-        t_rows, t_width, a.table_out_stride = _table(out[0], dev, "out tables")
-        if t_rows != n_rows or t_width != width:
-            _refuse(f"out tables must be [{n_rows}][{width}]")
-        a.refs_out = _int32(out[1], dev, (self.n_pages,), "out refs")
-        a.live = _int32(out[2], dev, (1,), "live")
+            out = t, r, live = tables.new_empty((n_rows, width)), torch.empty_like(refs), refs.new_empty(1)
+            a.tables_out, a.table_out_stride, a.refs_out, a.live = t.data_ptr(), width, r.data_ptr(), live.data_ptr()
+        else:
+            t_rows, t_width, a.table_out_stride = _table(out[0], dev, "out tables")
+            if t_rows != n_rows or t_width != width:
+                _refuse(f"out tables must be [{n_rows}][{width}]")
+            a.tables_out = out[0].data_ptr()
+            a.refs_out = _int32(out[1], dev, (self.n_pages,), "out refs")
+            a.live = _int32(out[2], dev, (1,), "live")
         a.n_rows, a.table_width = n_rows, width
-        a.tables, a.tables_out = tables.data_ptr(), out[0].data_ptr()
         stream = _stream_of(self._index)
-        keep = self._workspace(a, self._lib.cudallm_pages_workspace_bytes(self.n_pages, n_rows), stream)  # noqa: F841
+        keep = self._workspace(a, self._pages_size(n_rows), stream)  # noqa: F841
         self._run(self._call_compact, self._compact_ref, stream)
         return out
 
@@ -353,27 +378,30 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     a, ref = _beam_args()
     a.finished = None if finished is None else _int32(finished, dev, (groups, beams), "finished")
     if out is None:
-        out = (scores.new_empty((groups, keep)), *torch.empty((2, groups, keep), dtype=torch.int32, device=dev).unbind(0))
-    elif out[0].dtype is not torch.float32 or out[0].device != dev or tuple(out[0].shape) != (groups, keep) or not out[0].is_contiguous():
-        _refuse("out scores must be a contiguous fp32 tensor [groups][keep]")
-    a.out_scores = out[0].data_ptr()
-    a.out_parents = _int32(out[1], dev, (groups, keep), "out parents")
-    a.out_tokens = _int32(out[2], dev, (groups, keep), "out tokens")
+        parents, tokens = scores.new_empty((2, groups, keep), dtype=torch.int32).unbind(0)
+        out = best, parents, tokens = scores.new_empty((groups, keep)), parents, tokens
+        a.out_scores, a.out_parents, a.out_tokens = best.data_ptr(), parents.data_ptr(), tokens.data_ptr()
+    else:
+        if out[0].dtype is not torch.float32 or out[0].device != dev or out[0].shape != (groups, keep) or not out[0].is_contiguous():
+            _refuse("out scores must be a contiguous fp32 tensor [groups][keep]")
+        a.out_scores = out[0].data_ptr()
+        a.out_parents = _int32(out[1], dev, (groups, keep), "out parents")
+        a.out_tokens = _int32(out[2], dev, (groups, keep), "out tokens")
     a.x_dtype, a.n_groups, a.beams, a.keep, a.vocab, a.eos = x, groups, beams, keep, vocab, eos
     a.logits, a.row_stride, a.scores = logits.data_ptr(), row_stride, scores.data_ptr()
-    L = lib()
+    select, size = _beam_calls()
     index = dev.index
     stream = _stream_of(index)
     spaces = _shared.get(index)
     if spaces is None:
         spaces = _shared[index] = _Workspaces(dev)
-    w = spaces.get(stream, L.cudallm_beam_workspace_bytes(rows, vocab, keep))
+    w = spaces.get(stream, size(rows, vocab, keep))
     a.workspace, a.workspace_bytes = w.data_ptr(), w.numel()
     if torch.cuda.current_device() == index:
-        rc = L.cudallm_beam_select(ref, stream)
+        rc = select(ref, stream)
     else:
         with _OnDevice(index):
-            rc = L.cudallm_beam_select(ref, stream)
+            rc = select(ref, stream)
     if rc:
         check(rc)
     return out

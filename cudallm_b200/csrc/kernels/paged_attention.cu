@@ -691,59 +691,61 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
     copy_wait<0>();
 }
 
-// Joins the partials of items that were cut, in the order of their CTAs: block c those of the item that ends in CTA c's first
-// segment. Several warps share a head's partials; the loads of each are independent of each other.
-constexpr int kJoinWarps = 16;
+// Joins the partials of items that were cut, in the order of their CTAs: block (c, h) those of head h of the item that ends in CTA
+// c's first segment. The block's warps take every eighth partial; the loads of each are independent of each other.
+constexpr int kJoinWarps = 8;
 template <typename X, int HD>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Params p) {
     constexpr int V = HD / 32;  // dims of a lane
     __shared__ float warp_m[kJoinWarps], warp_l[kJoinWarps], warp_o[kJoinWarps][HD];
     grid_dep_wait();
     const int4 head = __ldcg(reinterpret_cast<const int4*>(p.endings + blockIdx.x));
-    if (head.x == 0) return;
-    const Ending e{head.x, head.y, head.z, 0, __ldcg(&p.endings[blockIdx.x].row0)};
+    const int parts = head.x, c0 = head.y, h = blockIdx.y;
+    if (parts == 0 || h >= head.z) return;
+    const long long row = __ldcg(&p.endings[blockIdx.x].row0) + h;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int ways = kJoinWarps / e.heads;  // warps of a head (16 heads at most)
-    const int h = warp / ways, way = warp % ways;
     float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.f;
-    auto part = [&](int c) { return p.parts + (static_cast<size_t>(e.c0 + c) * 2 + (c == 0)) * kSlotFloats; };
-    if (h < e.heads) {
-        for (int from = way; from < e.n; from += 32 * ways) {
-            const int mine = from + lane * ways;
-            const float pm = mine < e.n ? __ldcg(part(mine) + h) : -INFINITY, pl = mine < e.n ? __ldcg(part(mine) + 16 + h) : 0.f;
-            float top = fmaxf(m, pm);
+    auto part = [&](int c) { return p.parts + (static_cast<size_t>(c0 + c) * 2 + (c == 0)) * kSlotFloats; };
+    constexpr int kAtOnce = 8;
+    for (int from = warp; from < parts; from += kAtOnce * kJoinWarps) {
+        float pm[kAtOnce], pl[kAtOnce], po[kAtOnce][V];
 #pragma unroll
-            for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float ref = top == -INFINITY ? 0.f : top, old = exp2_fast(m - ref), w = exp2_fast(pm - ref);
-            float sum = w * pl;
+        for (int k = 0; k < kAtOnce; ++k) {
+            const int c = from + k * kJoinWarps;
+            pm[k] = -INFINITY;
+            if (c >= parts) continue;
+            const float* src = part(c);
+            pm[k] = __ldcg(src + h);
+            pl[k] = __ldcg(src + 16 + h);
+            src += 32 + h * HD + lane * V;
+            if constexpr (V == 2) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+                po[k][0] = v.x, po[k][1] = v.y;
+            } else {
 #pragma unroll
-            for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-            l = fmaf(l, old, sum);
-            m = top;
-#pragma unroll
-            for (int i = 0; i < V; ++i) o[i] *= old;
-            const int n = min(32, (e.n - from + ways - 1) / ways);
-#pragma unroll 8
-            for (int k = 0; k < n; ++k) {
-                const float* src = part(from + k * ways) + 32 + h * HD + lane * V;
-                const float f = __shfl_sync(0xffffffffu, w, k);
-                if constexpr (V == 2) {
-                    const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
-                    o[0] = fmaf(f, v.x, o[0]);
-                    o[1] = fmaf(f, v.y, o[1]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V / 4; ++i) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(src) + i);
-                        o[4 * i] = fmaf(f, v.x, o[4 * i]);
-                        o[4 * i + 1] = fmaf(f, v.y, o[4 * i + 1]);
-                        o[4 * i + 2] = fmaf(f, v.z, o[4 * i + 2]);
-                        o[4 * i + 3] = fmaf(f, v.w, o[4 * i + 3]);
-                    }
+                for (int i = 0; i < V; i += 4) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4*>(src + i));
+                    po[k][i] = v.x, po[k][i + 1] = v.y, po[k][i + 2] = v.z, po[k][i + 3] = v.w;
                 }
             }
+        }
+        float top = m;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, pm[k]);
+        const float ref = top == -INFINITY ? 0.f : top, old = exp2_fast(m - ref);
+        m = top;
+        l *= old;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] *= old;
+#pragma unroll
+        for (int k = 0; k < kAtOnce; ++k) {
+            if (from + k * kJoinWarps >= parts) break;
+            const float f = exp2_fast(pm[k] - ref);
+            l = fmaf(f, pl[k], l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = fmaf(f, po[k][i], o[i]);
         }
     }
     if (lane == 0) {
@@ -753,18 +755,18 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 #pragma unroll
     for (int i = 0; i < V; ++i) warp_o[warp][lane * V + i] = o[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < e.heads * HD; i += 32 * kJoinWarps) {
-        const int hh = i / HD, d = i % HD;
+    for (int d = threadIdx.x; d < p.head_dim; d += 32 * kJoinWarps) {
         float mm = -INFINITY, ll = 0.f, v = 0.f;
-        for (int w = hh * ways; w < (hh + 1) * ways; ++w) mm = fmaxf(mm, warp_m[w]);
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) mm = fmaxf(mm, warp_m[w]);
         const float ref = mm == -INFINITY ? 0.f : mm;
-        for (int w = hh * ways; w < (hh + 1) * ways; ++w) {
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
             const float f = exp2_fast(warp_m[w] - ref);
             ll = fmaf(f, warp_l[w], ll);
             v = fmaf(f, warp_o[w][d], v);
         }
-        const long long row = e.row0 + hh;
-        if (d < p.head_dim) static_cast<X*>(p.out)[row * p.head_dim + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
+        static_cast<X*>(p.out)[row * p.head_dim + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
         if (d == 0 && p.lse != nullptr) p.lse[row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
     }
 }
@@ -823,7 +825,7 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
         launch_kernel(kernel, dim3(grid), dim3(kThreads), smem, stream, false, p);
         // Items of up to kUnit tiles are cut only where equal shares cut them, which takes more tiles than there are CTAs x kUnit.
         const bool can_cut = (cap + S::kTile - 1) / S::kTile > kUnit || static_cast<long long>(p.n_seq) * p.items > grid;
-        if (can_cut) launch_kernel(join_kernel<X, HD>, dim3(grid), dim3(32 * kJoinWarps), 0, stream, true, p);
+        if (can_cut) launch_kernel(join_kernel<X, HD>, dim3(grid, std::min(p.group, S::kHeads)), dim3(32 * kJoinWarps), 0, stream, true, p);
     }
 }
 

@@ -244,10 +244,10 @@ class PagedCache:
         a = self._attend
         a.lens = _int32(lens, self.device, (n,), "lens")
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = q.new_empty(n, heads, self.head_dim)
         elif out.dtype is not q.dtype or out.device != self.device or out.shape != q.shape or not out.is_contiguous():
             _refuse("out must be contiguous, with q's shape and type")
-        lse = q.new_empty((n, heads), dtype=torch.float32) if with_lse else None
+        lse = None if not with_lse else q.new_empty(n, heads, dtype=torch.float32)
         a.layer, a.x_dtype, a.n_seq, a.n_heads, a.table_width, a.window = layer, x, n, heads, width, window
         a.scale = self._scale if scale is None else scale
         a.q, a.q_seq_stride, a.q_head_stride = q.data_ptr(), a_seq, a_head
@@ -279,7 +279,7 @@ class PagedCache:
             if nq != n:
                 _refuse("q, k and v must have the same number of tokens")
             if out is None:
-                out = torch.empty_like(q, memory_format=torch.contiguous_format)
+                out = q.new_empty(n, heads, dim)
                 a.out_token_stride, a.out_head_stride = heads * dim, dim
             elif out.shape != q.shape:
                 _refuse("out must have q's shape")
@@ -317,7 +317,7 @@ class PagedCache:
         a.parents = _int32(parents, dev, (n_out,), "parents")
         a.tables = tables.data_ptr()
         if out is None:
-            out = t, n, r, missing = tables.new_empty((n_out, width)), torch.empty_like(parents), torch.empty_like(refs), refs.new_empty(1)
+            out = t, n, r, missing = tables.new_empty(n_out, width), torch.empty_like(parents), torch.empty_like(refs), refs.new_empty(1)
             a.tables_out, a.table_out_stride = t.data_ptr(), width
             a.lens_out, a.refs_out, a.missing = n.data_ptr(), r.data_ptr(), missing.data_ptr()
         else:
@@ -342,7 +342,7 @@ class PagedCache:
         a.refs = _int32(refs, dev, (self.n_pages,), "refs")
         a.tables = tables.data_ptr()
         if out is None:
-            out = t, r, live = tables.new_empty((n_rows, width)), torch.empty_like(refs), refs.new_empty(1)
+            out = t, r, live = tables.new_empty(n_rows, width), torch.empty_like(refs), refs.new_empty(1)
             a.tables_out, a.table_out_stride, a.refs_out, a.live = t.data_ptr(), width, r.data_ptr(), live.data_ptr()
         else:
             t_rows, t_width, a.table_out_stride = _table(out[0], dev, "out tables")
@@ -378,8 +378,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     a, ref = _beam_args()
     a.finished = None if finished is None else _int32(finished, dev, (groups, beams), "finished")
     if out is None:
-        parents, tokens = scores.new_empty((2, groups, keep), dtype=torch.int32).unbind(0)
-        out = best, parents, tokens = scores.new_empty((groups, keep)), parents, tokens
+        best = scores.new_empty(groups, keep)
+        parents = torch.empty_like(best, dtype=torch.int32)
+        tokens = torch.empty_like(parents)
+        out = best, parents, tokens
         a.out_scores, a.out_parents, a.out_tokens = best.data_ptr(), parents.data_ptr(), tokens.data_ptr()
     else:
         if out[0].dtype is not torch.float32 or out[0].device != dev or out[0].shape != (groups, keep) or not out[0].is_contiguous():

@@ -65,6 +65,13 @@ __device__ __forceinline__ int block_sum(int v, int* sm) {
     return s;
 }
 
+// 2^x to 22 bits, which a sum of thousands of them averages out; exp(x) = 2^(x log2(e)).
+__device__ __forceinline__ float exp_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    return y;
+}
+
 template <typename X>
 __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const __grid_constant__ cudallm_beam_args a, uint64_t* lists, float2* stats, int chunks,
                                                               bool wide) {
@@ -127,7 +134,7 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const __grid_const
     const float ref = m == -INFINITY ? 0.f : m;
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) s += expf(v[j] - ref);
+    for (int j = 0; j < kEach; ++j) s += exp_fast(v[j] - ref);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
     if (lane == 0) {
@@ -152,45 +159,46 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const __grid_const
     }
     __syncthreads();
     uint32_t bound = sm_bound;
-    int above = 0;
+    auto push = [&](int j) {
+        const int p = atomicAdd(&sm_count, 1);
+        if (p < kList) list[p] = static_cast<uint64_t>(bits[j]) << 32 | static_cast<uint32_t>(~(c0 + at(j)));
+    };
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) above += bits[j] >= bound;
-    int count = block_sum<kThreads>(above, sm_n);
-    uint32_t last = kAll;  // of the logits with exactly `bound`, those up to this place are taken
-    if (count > kList) {
-        // The keep-th value, then how far its ties go.
+    for (int j = 0; j < kEach; ++j)
+        if (bits[j] >= bound) push(j);
+    __syncthreads();
+    if (sm_count > kList) {
+        // Too many ties to list: the keep-th value, then how far its ties go.
         bound = 0;
 #pragma unroll 1
         for (int bit = 31; bit >= 0; --bit) {
             const uint32_t test = bound | 1u << bit;
-            above = 0;
+            int above = 0;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) above += bits[j] >= test;
             if (block_sum<kThreads>(above, sm_n) >= a.keep) bound = test;
         }
-        above = 0;
+        int above = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) above += bits[j] > bound;
         const int ties = a.keep - block_sum<kThreads>(above, sm_n);  // wanted: 1 or more
-        last = 0;
+        uint32_t last = 0;  // the largest place with fewer ties before it
 #pragma unroll 1
-        for (int bit = 11; bit >= 0; --bit) {  // the largest place with fewer ties before it
+        for (int bit = 11; bit >= 0; --bit) {
             const uint32_t test = last | 1u << bit;
             above = 0;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) above += bits[j] == bound && at(j) < static_cast<int>(test);
             if (block_sum<kThreads>(above, sm_n) < ties) last = test;
         }
-        count = a.keep;
-    }
+        if (threadIdx.x == 0) sm_count = 0;
+        __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        if (bits[j] > bound || (bits[j] == bound && static_cast<uint32_t>(at(j)) <= last)) {
-            list[atomicAdd(&sm_count, 1)] = static_cast<uint64_t>(bits[j]) << 32 | static_cast<uint32_t>(~(c0 + at(j)));
-        }
+        for (int j = 0; j < kEach; ++j)
+            if (bits[j] > bound || (bits[j] == bound && static_cast<uint32_t>(at(j)) <= last)) push(j);
     }
     __syncthreads();
-    count = min(sm_count, kList);
+    const int count = min(sm_count, kList);
     if (threadIdx.x < count) {
         const uint64_t key = list[threadIdx.x];
         int rank = 0;

@@ -6,6 +6,8 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <cstdint>
 #include <utility>
 
 #include "common/check.h"
@@ -26,6 +28,16 @@ void launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
     cfg.attrs = attr;
     cfg.numAttrs = pdl ? 1 : 0;
     CLLM_CUDA(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
+}
+
+// Lets a kernel use `bytes` of shared memory on the current device; `allowed` holds the devices where it may already (a bit each).
+template <typename... KArgs>
+void allow_shared(void (*kernel)(KArgs...), int bytes, std::atomic<uint64_t>& allowed) {
+    int dev = 0;
+    CLLM_CUDA(cudaGetDevice(&dev));
+    if (dev < 64 && (allowed.load() >> dev & 1)) return;
+    CLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    if (dev < 64) allowed.fetch_or(1ull << dev);
 }
 
 }  // namespace cudallm

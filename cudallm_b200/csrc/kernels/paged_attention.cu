@@ -802,12 +802,7 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
     p.row_step = pg.token_stride * 2 * (32 / (HD / 8));
     auto kernel = attend_kernel<X, KV, HD, HG>;
     static std::atomic<uint64_t> allowed{0};  // devices on which this kernel may use its shared memory
-    int dev = 0;
-    CLLM_CUDA(cudaGetDevice(&dev));
-    if (dev >= 64 || !(allowed.load() >> dev & 1)) {
-        CLLM_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kFixed + 4 * (kMaxRows + 1)));
-        if (dev < 64) allowed.fetch_or(1ull << dev);
-    }
+    allow_shared(kernel, S::kFixed + 4 * (kMaxRows + 1), allowed);
     const long long cap = static_cast<long long>(a.table_width) * pg.page_size;
     const long long row_tiles = std::max(1LL, (cap + S::kTile - 1) / S::kTile * p.items);  // most tiles of a sequence
     CLLM_REQUIRE(row_tiles <= (1LL << 31), "cudallm_paged_attend: the tables are too wide");

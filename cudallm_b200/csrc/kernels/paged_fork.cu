@@ -1,10 +1,15 @@
 // Bookkeeping of a paged cache's sequences: forking (sharing, copy on write, freeing, new pages) and compaction.
 //
-// Both run as a plan kernel, whose first block decides who gets which page (all of it integer prefix sums, so the result
-// does not depend on any order of threads), and a kernel over the whole GPU, in place when the plan is done, that moves
-// the tokens of every layer and writes tables and references. The moves read and write each byte once and HBM bounds
-// them; with few of them the plan's chain of dependent loads (parent, length, entry, references) does.
+// A plan decides who gets which page (all of it integer prefix sums, so the result does not depend on any order of
+// threads); then the tokens of every layer move and tables and references are written. The moves read and write each
+// byte once and HBM bounds them; with few of them the plan's chain of dependent loads (parent, length, entry,
+// references) does.
+//
+// One launch where plan and moves are small: every block makes the whole plan for itself, in shared memory, which costs no
+// more time than one block making it, and moves its share (the caller's thread needs 5 us instead of 8.5). Otherwise two: a plan kernel into
+// the workspace and a move kernel over the GPU, in place when the plan is done.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "common/check.h"
@@ -65,17 +70,17 @@ __device__ __forceinline__ void load_refs(const int* refs, int p, int n, int non
 }
 
 // One warp copies `tokens` tokens of one head of one page of one layer, of k and of v.
+template <int AT_ONCE>
 __device__ __forceinline__ void copy_head(const cudallm_pages& pg, FastDiv by_row, int layer, int head, int src, int dst, int tokens) {
     const int per_row = pg.head_dim / 8, n = tokens * per_row, lane = threadIdx.x & 31;  // 16-byte words
     const long long base = layer * pg.layer_stride + head * pg.head_stride;
     const uint16_t *ks = static_cast<const uint16_t*>(pg.k) + base + src * pg.page_stride, *vs = static_cast<const uint16_t*>(pg.v) + base + src * pg.page_stride;
     uint16_t *kd = static_cast<uint16_t*>(pg.k) + base + dst * pg.page_stride, *vd = static_cast<uint16_t*>(pg.v) + base + dst * pg.page_stride;
-    constexpr int kAtOnce = 4;
-    for (int c0 = lane; c0 < n; c0 += 32 * kAtOnce) {
-        uint4 k[kAtOnce], v[kAtOnce];
-        long long at[kAtOnce];
+    for (int c0 = lane; c0 < n; c0 += 32 * AT_ONCE) {
+        uint4 k[AT_ONCE], v[AT_ONCE];
+        long long at[AT_ONCE];
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
+        for (int i = 0; i < AT_ONCE; ++i) {
             const int c = c0 + 32 * i;
             if (c >= n) break;
             const int t = div_by(c, by_row);
@@ -84,7 +89,7 @@ __device__ __forceinline__ void copy_head(const cudallm_pages& pg, FastDiv by_ro
             v[i] = *reinterpret_cast<const uint4*>(vs + at[i]);
         }
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
+        for (int i = 0; i < AT_ONCE; ++i) {
             if (c0 + 32 * i >= n) break;
             *reinterpret_cast<uint4*>(kd + at[i]) = k[i];
             *reinterpret_cast<uint4*>(vd + at[i]) = v[i];
@@ -99,31 +104,34 @@ struct OutRow {
 };
 struct OldRow {
     int full, held, children, kept;  // full pages, entries held, children, whether a child takes over what follows the full pages
+    int open;                        // the page after the full ones, or -1
 };
 struct Copy {
     int src, dst, tokens, pad;
 };
 struct ForkPlan {
-    int* totals;  // new pages found, copies
+    int* totals;  // new pages found, copies, pages missing
     OutRow* out;
-    OldRow* old;
     Copy* copies;
-    int *fresh, *children, *first, *found;
+    OldRow* old;
+    int *fresh, *counters, *found;
 };
+constexpr int kOneRows = 512, kOneFound = 2048;  // what a plan in shared memory has room for
+constexpr int kOneEntries = 16384;               // and of the tables, which one block writes then
+constexpr long long kOneHeads = 8192;            // heads of pages that may move: with more, two launches and smaller blocks gain 2 to 6 us
 
-// Bytes of a plan for that many rows, and its parts in a workspace.
-__host__ __device__ inline size_t fork_plan_bytes(int n_pages, int rows) { return 256 + (3 * 16 + 3 * 4) * static_cast<size_t>(rows) + 4 * static_cast<size_t>(n_pages); }
-inline ForkPlan fork_plan(void* workspace, int rows) {
-    char* p = static_cast<char*>(workspace);
+// Bytes of a plan for that many rows and new pages, and its parts in 16-byte aligned memory.
+__host__ __device__ inline size_t fork_plan_bytes(int rows, int found) { return 16 + (2 * 16 + 20 + 3 * 4) * static_cast<size_t>(rows) + 4 * static_cast<size_t>(found); }
+__host__ __device__ inline ForkPlan fork_plan(void* memory, int rows, int found) {
+    char* p = static_cast<char*>(memory);
     ForkPlan s;
     s.totals = reinterpret_cast<int*>(p);
-    s.out = reinterpret_cast<OutRow*>(p + 256);
-    s.old = reinterpret_cast<OldRow*>(s.out + rows);
-    s.copies = reinterpret_cast<Copy*>(s.old + rows);
-    s.fresh = reinterpret_cast<int*>(s.copies + rows);
-    s.children = s.fresh + rows;
-    s.first = s.children + rows;
-    s.found = s.first + rows;
+    s.out = reinterpret_cast<OutRow*>(p + 16);
+    s.copies = reinterpret_cast<Copy*>(s.out + rows);
+    s.found = reinterpret_cast<int*>(s.copies + rows);
+    s.old = reinterpret_cast<OldRow*>(s.found + found);
+    s.fresh = reinterpret_cast<int*>(s.old + rows);
+    s.counters = s.fresh + rows;
     return s;
 }
 
@@ -132,21 +140,13 @@ __device__ __forceinline__ int row_len(const cudallm_pages& pg, const cudallm_fo
     return static_cast<int>(min(static_cast<long long>(max(a.lens[r], 0)), cap));
 }
 
-// Block 0 plans; the others copy the references, which the move kernel then changes.
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
-                                                                 bool wide) {
-    extern __shared__ int counters[];  // children and first child of up to kSharedRows rows
+// The plan of a fork, by all threads of a block. `counters`: room for two ints for each of n_rows. Ends with a barrier.
+__device__ __forceinline__ void plan_fork(const cudallm_pages& pg, const cudallm_fork_args& a, const ForkPlan& s, int* counters, bool wide) {
     __shared__ int sm[32];
     __shared__ unsigned long long over;
-    grid_dep_launch();
-    if (blockIdx.x > 0) {
-        for (int p = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; p < pg.n_pages; p += (gridDim.x - 1) * kPlanThreads) a.refs_out[p] = a.refs[p];
-        return;
-    }
     int refs[kEach];  // of the first pass, under way while the rows are looked at
     load_refs(a.refs, threadIdx.x * kEach, pg.n_pages, 1, wide, refs);
-    int* children = a.n_rows <= kSharedRows ? counters : s.children;
-    int* first = a.n_rows <= kSharedRows ? counters + a.n_rows : s.first;
+    int *children = counters, *first = counters + a.n_rows;
     for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {
         children[r] = 0;
         first[r] = INT_MAX;
@@ -163,9 +163,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_co
     for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {
         const int full = row_len(pg, a, r) / pg.page_size;
         const int* row = a.tables + r * a.table_stride;
-        int held = full;
-        while (held < a.table_width && is_page(row[held], pg.n_pages)) ++held;
-        s.old[r] = {full, held, 0, held > full && a.refs[row[full]] == 1};
+        int held = full, open = -1;
+        for (; held < a.table_width; ++held) {
+            const int e = row[held];
+            if (!is_page(e, pg.n_pages)) break;
+            if (held == full) open = e;
+        }
+        s.old[r] = {full, held, 0, open >= 0 && a.refs[open] == 1, open};
     }
     __syncthreads();
     for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {  // a thread's own rows
@@ -225,9 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_co
                 const OldRow old = s.old[o.parent];
                 const int tail = o.len - old.full * pg.page_size;
                 const bool keeps = old.kept && first[o.parent] == i;
-                if (!keeps && tail > 0 && old.held > old.full && s.fresh[i] > 0 && o.start < found) {
-                    c = {a.tables[o.parent * a.table_stride + old.full], s.found[o.start], tail, 0};
-                }
+                if (!keeps && tail > 0 && old.open >= 0 && s.fresh[i] > 0 && o.start < found) c = {old.open, s.found[o.start], tail, 0};
             }
         }
         int total;
@@ -239,66 +241,111 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_co
         s.totals[0] = found;
         s.totals[1] = copies;
         const unsigned long long missing = over + static_cast<unsigned long long>(base - found);
-        *a.missing = static_cast<int>(min(missing, static_cast<unsigned long long>(INT_MAX)));
+        s.totals[2] = static_cast<int>(min(missing, static_cast<unsigned long long>(INT_MAX)));
+    }
+    __syncthreads();
+}
+
+// Rows of the outputs, and the references that the parents' pages lose or gain: thread `me` of `threads` takes entries.
+__device__ __forceinline__ void fork_rows(const cudallm_pages& pg, const cudallm_fork_args& a, const ForkPlan& s, int rows, long long me, long long threads) {
+    const int n_found = s.totals[0];
+    const long long entries = static_cast<long long>(rows) * a.table_width;
+    for (long long x = me; x < entries; x += threads) {
+        const int i = static_cast<int>(x / a.table_width), j = static_cast<int>(x % a.table_width);
+        if (i < a.n_rows) {
+            const OldRow old = s.old[i];
+            const int gain = j < old.full ? old.children - 1 : old.kept ? 0 : -1;
+            if (j < old.held && gain != 0) {
+                const int p = a.tables[i * a.table_stride + j];
+                if (is_page(p, pg.n_pages)) atomicAdd(&a.refs_out[p], gain);
+            }
+        }
+        if (i < a.n_out) {
+            const OutRow o = s.out[i];
+            int e = -1;
+            if (o.parent >= 0 && j < o.from) {
+                e = a.tables[o.parent * a.table_stride + j];
+                if (!is_page(e, pg.n_pages)) e = -1;
+            } else if (j < o.from + s.fresh[i] && o.start + j - o.from < n_found) {
+                e = s.found[o.start + j - o.from];
+                atomicAdd(&a.refs_out[e], 1);
+            }
+            a.tables_out[i * a.table_out_stride + j] = e;
+        }
+    }
+    for (long long i = me; i < a.n_out; i += threads) a.lens_out[i] = s.out[i].len;
+}
+
+// Copies: warp `warp` of `warps` takes every so manieth head of a page.
+template <int AT_ONCE>
+__device__ __forceinline__ void fork_copies(const cudallm_pages& pg, const ForkPlan& s, FastDiv by_row, long long warp, long long warps) {
+    const long long units = static_cast<long long>(s.totals[1]) * pg.n_layers * pg.n_kv_heads;
+    for (long long u = warp; u < units; u += warps) {
+        const int head = static_cast<int>(u % pg.n_kv_heads), layer = static_cast<int>(u / pg.n_kv_heads % pg.n_layers);
+        const Copy c = s.copies[u / pg.n_kv_heads / pg.n_layers];
+        copy_head<AT_ONCE>(pg, by_row, layer, head, c.src, c.dst, c.tokens);
     }
 }
 
-// The first `rows` blocks: row i of the outputs, and the references that parent row i's pages lose or gain. The other blocks' warps
-// each copy heads of pages.
-__global__ void __launch_bounds__(kMoveThreads) fork_move_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
-                                                                 int rows, FastDiv by_row) {
-    grid_dep_wait();
-    const int i = blockIdx.x;
-    if (i >= rows) {
-        const long long units = static_cast<long long>(s.totals[1]) * pg.n_layers * pg.n_kv_heads;
-        const long long step = static_cast<long long>(gridDim.x - rows) * (kMoveThreads / 32);
-        for (long long u = static_cast<long long>(i - rows) * (kMoveThreads / 32) + threadIdx.x / 32; u < units; u += step) {
-            const int head = static_cast<int>(u % pg.n_kv_heads), layer = static_cast<int>(u / pg.n_kv_heads % pg.n_layers);
-            const Copy c = s.copies[u / pg.n_kv_heads / pg.n_layers];
-            copy_head(pg, by_row, layer, head, c.src, c.dst, c.tokens);
-        }
+// Block 0 plans; the others copy the references, which the move kernel then changes.
+__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
+                                                                 bool wide) {
+    extern __shared__ int shared_counters[];
+    grid_dep_launch();
+    if (blockIdx.x > 0) {
+        for (int p = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; p < pg.n_pages; p += (gridDim.x - 1) * kPlanThreads) a.refs_out[p] = a.refs[p];
         return;
     }
-    if (i < a.n_rows) {
-        const OldRow old = s.old[i];
-        for (int j = threadIdx.x; j < old.held; j += kMoveThreads) {
-            const int p = a.tables[i * a.table_stride + j];
-            const int gain = j < old.full ? old.children - 1 : old.kept ? 0 : -1;
-            if (gain != 0 && is_page(p, pg.n_pages)) atomicAdd(&a.refs_out[p], gain);
-        }
+    plan_fork(pg, a, s, a.n_rows <= kSharedRows ? shared_counters : s.counters, wide);
+    if (threadIdx.x == 0) *a.missing = s.totals[2];
+}
+
+// The first `writers` blocks write rows; the others' warps copy.
+__global__ void __launch_bounds__(kMoveThreads) fork_move_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
+                                                                 int rows, int writers, FastDiv by_row) {
+    grid_dep_wait();
+    if (static_cast<int>(blockIdx.x) < writers) {
+        fork_rows(pg, a, s, rows, static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x, static_cast<long long>(writers) * kMoveThreads);
+    } else {
+        constexpr int kWarps = kMoveThreads / 32;
+        fork_copies<4>(pg, s, by_row, static_cast<long long>(blockIdx.x - writers) * kWarps + threadIdx.x / 32, static_cast<long long>(gridDim.x - writers) * kWarps);
     }
-    if (i >= a.n_out) return;
-    const OutRow o = s.out[i];
-    const int n_found = s.totals[0], fresh = s.fresh[i];
-    const int* old = a.tables + static_cast<long long>(max(o.parent, 0)) * a.table_stride;
-    for (int j = threadIdx.x; j < a.table_width; j += kMoveThreads) {
-        int e = -1;
-        if (o.parent >= 0 && j < o.from) {
-            e = is_page(old[j], pg.n_pages) ? old[j] : -1;
-        } else if (j < o.from + fresh && o.start + j - o.from < n_found) {
-            e = s.found[o.start + j - o.from];
-            atomicAdd(&a.refs_out[e], 1);
-        }
-        a.tables_out[i * a.table_out_stride + j] = e;
+}
+
+// The whole fork: block 0 writes the rows, the other blocks copy.
+__global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, int rows, FastDiv by_row,
+                                                            bool wide) {
+    extern __shared__ __align__(16) char room[];
+    const ForkPlan s = fork_plan(room, rows, kOneFound);
+    if (blockIdx.x == 0) {
+        for (int p = threadIdx.x; p < pg.n_pages; p += kPlanThreads) a.refs_out[p] = a.refs[p];
     }
-    if (threadIdx.x == 0) a.lens_out[i] = o.len;
+    plan_fork(pg, a, s, s.counters, wide);
+    if (blockIdx.x == 0) {
+        if (threadIdx.x == 0) *a.missing = s.totals[2];
+        fork_rows(pg, a, s, rows, threadIdx.x, kPlanThreads);
+    } else {
+        constexpr int kWarps = kPlanThreads / 32;
+        fork_copies<2>(pg, s, by_row, static_cast<long long>(blockIdx.x - 1) * kWarps + threadIdx.x / 32, static_cast<long long>(gridDim.x - 1) * kWarps);
+    }
 }
 
 // ---- compact ---------------------------------------------------------------------------------------
 
 struct CompactPlan {
     int* totals;          // pages in use, moves
-    int *to, *src, *dst;  // new place of a page that moves; the moves
+    int *to, *src, *dst;  // new place of a page that moves; the moves (at most half of the pages: none moves onto one that stays)
 };
-inline CompactPlan compact_plan(void* workspace, int n_pages) {
-    int* p = static_cast<int*>(workspace);
-    return {p, p + 64, p + 64 + n_pages, p + 64 + 2 * static_cast<size_t>(n_pages)};
+__host__ __device__ inline size_t compact_plan_bytes(int n_pages) { return 16 + 8 * static_cast<size_t>(n_pages); }
+__host__ __device__ inline CompactPlan compact_plan(void* memory, int n_pages) {
+    int* p = static_cast<int*>(memory);
+    return {p, p + 4, p + 4 + n_pages, p + 4 + n_pages + n_pages / 2};
 }
+constexpr int kOnePages = kPass;  // pages of a plan in shared memory
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
-                                                                    bool wide) {
+// The plan of a compaction, by all threads of a block. Ends with a barrier.
+__device__ __forceinline__ void plan_compact(const cudallm_pages& pg, const cudallm_compact_args& a, const CompactPlan& s, bool wide) {
     __shared__ int sm[32];
-    grid_dep_launch();
     int refs[kEach], live = 0;
     for (int p0 = 0; p0 < pg.n_pages; p0 += kPass) {
         load_refs(a.refs, p0 + threadIdx.x * kEach, pg.n_pages, 0, wide, refs);
@@ -331,15 +378,21 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid
     if (threadIdx.x == 0) {
         s.totals[0] = live;
         s.totals[1] = movers;
-        *a.live = live;
     }
+    __syncthreads();
 }
 
-__global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
-                                                                    FastDiv by_row) {
-    grid_dep_wait();
+// Carries a plan out: thread `me` of `threads`.
+template <int AT_ONCE>
+__device__ __forceinline__ void move_compact(const cudallm_pages& pg, const cudallm_compact_args& a, const CompactPlan& s, FastDiv by_row, long long me, long long threads) {
     const int live = s.totals[0];
-    const long long threads = static_cast<long long>(gridDim.x) * kMoveThreads, me = static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x;
+    if (me == 0) *a.live = live;
+    const long long units = static_cast<long long>(s.totals[1]) * pg.n_layers * pg.n_kv_heads;
+    for (long long u = me / 32; u < units; u += threads / 32) {
+        const int head = static_cast<int>(u % pg.n_kv_heads), layer = static_cast<int>(u / pg.n_kv_heads % pg.n_layers);
+        const int k = static_cast<int>(u / pg.n_kv_heads / pg.n_layers);
+        copy_head<AT_ONCE>(pg, by_row, layer, head, s.src[k], s.dst[k], pg.page_size);
+    }
     for (long long p = me; p < pg.n_pages; p += threads) {
         const int r = a.refs[p];
         if (p >= live) a.refs_out[p] = 0;
@@ -351,12 +404,26 @@ __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const __grid
         const int p = a.tables[r * a.table_stride + j];
         a.tables_out[r * a.table_out_stride + j] = !is_page(p, pg.n_pages) ? -1 : p >= live && a.refs[p] > 0 ? s.to[p] : p;
     }
-    const long long units = static_cast<long long>(s.totals[1]) * pg.n_layers * pg.n_kv_heads;
-    for (long long u = me / 32; u < units; u += threads / 32) {
-        const int head = static_cast<int>(u % pg.n_kv_heads), layer = static_cast<int>(u / pg.n_kv_heads % pg.n_layers);
-        const int k = static_cast<int>(u / pg.n_kv_heads / pg.n_layers);
-        copy_head(pg, by_row, layer, head, s.src[k], s.dst[k], pg.page_size);
-    }
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
+                                                                    bool wide) {
+    grid_dep_launch();
+    plan_compact(pg, a, s, wide);
+}
+
+__global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
+                                                                    FastDiv by_row) {
+    grid_dep_wait();
+    move_compact<4>(pg, a, s, by_row, static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x, static_cast<long long>(gridDim.x) * kMoveThreads);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, FastDiv by_row,
+                                                               bool wide) {
+    extern __shared__ __align__(16) char room[];
+    const CompactPlan s = compact_plan(room, pg.n_pages);
+    plan_compact(pg, a, s, wide);
+    move_compact<2>(pg, a, s, by_row, static_cast<long long>(blockIdx.x) * kPlanThreads + threadIdx.x, static_cast<long long>(gridDim.x) * kPlanThreads);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -365,28 +432,49 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 size_t pages_workspace_bytes(int n_pages, int rows) {
     if (n_pages < 1 || rows < 0 || rows > kMaxPageRows) return 0;
-    return std::max(fork_plan_bytes(n_pages, rows), 256 + 12 * static_cast<size_t>(n_pages));
+    return std::max(fork_plan_bytes(rows, n_pages), compact_plan_bytes(n_pages));
 }
 
 void launch_paged_fork(const cudallm_pages& pg, const cudallm_fork_args& a, cudaStream_t stream) {
     const int rows = std::max(a.n_rows, a.n_out), sms = num_sms();
-    const ForkPlan s = fork_plan(a.workspace, rows);
+    const FastDiv by_row = fast_div(pg.head_dim / 8);
+    const bool wide = aligned16(a.refs);
+    const long long heads = static_cast<long long>(a.n_out) * pg.n_layers * pg.n_kv_heads;  // most that are copied
+    const long long most_new = a.n_out * (2LL + a.room / pg.page_size);
+    if (pg.n_pages <= kPass && rows <= kOneRows && most_new <= kOneFound && static_cast<long long>(rows) * a.table_width <= kOneEntries &&
+        heads <= kOneHeads) {
+        constexpr int kWarps = kPlanThreads / 32;
+        const int blocks = 1 + static_cast<int>(std::min<long long>(sms - 1, std::max<long long>(1, (heads + kWarps - 1) / kWarps)));
+        launch_kernel(fork_kernel, dim3(blocks), dim3(kPlanThreads), fork_plan_bytes(rows, kOneFound), stream, false, pg, a, rows, by_row, wide);
+        return;
+    }
+    const ForkPlan s = fork_plan(a.workspace, rows, pg.n_pages);
     const int copiers = std::min(sms, (pg.n_pages + kPlanThreads - 1) / kPlanThreads);  // of the references
     const size_t smem = a.n_rows <= kSharedRows ? 8 * static_cast<size_t>(a.n_rows) : 0;
-    launch_kernel(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), smem, stream, false, pg, a, s, aligned16(a.refs));
+    launch_kernel(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), smem, stream, false, pg, a, s, wide);
     if (rows == 0) return;
-    const long long heads = static_cast<long long>(a.n_out) * pg.n_layers * pg.n_kv_heads;
     const int movers = static_cast<int>(std::min<long long>(8LL * sms, (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
-    launch_kernel(fork_move_kernel, dim3(rows + movers), dim3(kMoveThreads), 0, stream, true, pg, a, s, rows, fast_div(pg.head_dim / 8));
+    const long long entries = static_cast<long long>(rows) * a.table_width;
+    const int writers = static_cast<int>(std::min<long long>(sms, 1 + entries / (4 * kMoveThreads)));
+    launch_kernel(fork_move_kernel, dim3(writers + movers), dim3(kMoveThreads), 0, stream, true, pg, a, s, rows, writers, by_row);
 }
 
 void launch_paged_compact(const cudallm_pages& pg, const cudallm_compact_args& a, cudaStream_t stream) {
+    const FastDiv by_row = fast_div(pg.head_dim / 8);
+    const bool wide = aligned16(a.refs);
+    const long long heads = static_cast<long long>(pg.n_pages / 2) * pg.n_layers * pg.n_kv_heads;  // most that move
+    if (pg.n_pages <= kOnePages && heads <= kOneHeads) {
+        const size_t smem = compact_plan_bytes(pg.n_pages);
+        static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
+        allow_shared(compact_kernel, static_cast<int>(compact_plan_bytes(kOnePages)), allowed);
+        const long long most = 1 + (heads + kPlanThreads / 32 - 1) / (kPlanThreads / 32);
+        launch_kernel(compact_kernel, dim3(static_cast<int>(std::min<long long>(num_sms(), most))), dim3(kPlanThreads), smem, stream, false, pg, a, by_row, wide);
+        return;
+    }
     const CompactPlan s = compact_plan(a.workspace, pg.n_pages);
-    launch_kernel(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, false, pg, a, s, aligned16(a.refs));
-    // No page moves onto another that stays, so at most half of the pages move.
-    const long long heads = static_cast<long long>(pg.n_pages / 2) * pg.n_layers * pg.n_kv_heads;
+    launch_kernel(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, false, pg, a, s, wide);
     const int blocks = static_cast<int>(std::min<long long>(8LL * num_sms(), 1 + (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
-    launch_kernel(compact_move_kernel, dim3(blocks), dim3(kMoveThreads), 0, stream, true, pg, a, s, fast_div(pg.head_dim / 8));
+    launch_kernel(compact_move_kernel, dim3(blocks), dim3(kMoveThreads), 0, stream, true, pg, a, s, by_row);
 }
 
 }  // namespace cudallm

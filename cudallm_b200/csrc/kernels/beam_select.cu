@@ -5,13 +5,14 @@
 // Within a row candidates rank as (logit, then lower token), so the `keep` best by logit of each chunk of a row are the
 // only ones that can be among the group's.
 //
-// chunk kernel: one block per 4096 logits, which stay in registers (one read of the logits, what bounds the operator at
+// chunk stage: one block per 4096 logits, which stay in registers (one read of the logits, what bounds the operator at
 //   many rows). It leaves their maximum, their sum of exponentials and the sorted keys of their `keep` best. A lower
 //   bound of the keep-th best is the keep-th largest of the maxima of 512 pieces; the few logits above it are ranked by
 //   counting. Where more than 256 are above it (ties, a masked vocabulary) the keep-th key itself is
 //   searched bit by bit over value and token.
-// group kernel: one block per group, in place when the chunks are done. It joins the rows' sums and ranks the chunks'
-//   lists' candidates in the same way.
+// group stage: joins the rows' sums and ranks the lists' candidates in the same way. Up to 256 chunks the last block of a
+//   group to finish does it; with more, a block for each group in a second launch, in place when the chunks are done (4 rows x
+//   128256: 17.7 us a call with one launch, 21.7 with two, of which the GPU needs 11 and 9; 64 rows: 24.8 and 22.2).
 #include <cmath>
 
 #include "common/check.h"
@@ -31,6 +32,7 @@ constexpr int kChunk = kThreads * kEach;
 constexpr int kList = 256;  // candidates above the bound that are ranked by counting
 constexpr int kGroupThreads = 512;
 constexpr int kGroupList = 512;
+constexpr int kOneLaunch = 256;  // chunks of a call with a single launch
 constexpr unsigned kAll = 0xffffffffu;
 
 // Rank bits of a logit: not a number counts as -inf, -0 as 0.
@@ -65,6 +67,131 @@ __device__ __forceinline__ int block_sum(int v, int* sm) {
     return s;
 }
 
+struct Best {
+    uint32_t bits;  // of the candidate
+    int row;        // beam in the group
+    uint64_t key;   // logit and token
+};
+__device__ __forceinline__ bool better(const Best& a, const Best& b) {
+    return a.bits != b.bits ? a.bits > b.bits : a.row != b.row ? a.row < b.row : a.key > b.key;
+}
+
+constexpr int kSamples = 512;  // what bound_of takes
+template <int THREADS>
+struct GroupRoom {
+    float lse[kMaxBeams], score[kMaxBeams];
+    Best list[kGroupList], best[THREADS / 32];
+    uint32_t samples[kSamples], bound;
+    int count;
+};
+
+// The best of group g, from its rows' lists and sums, by all threads of a block.
+template <int THREADS>
+__device__ void select_group(const cudallm_beam_args& a, const uint64_t* lists, const float2* stats, int chunks, int g, GroupRoom<THREADS>& sm) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) sm.count = 0;
+    for (int w = warp; w < a.beams; w += THREADS / 32) {
+        const float2* st = stats + (static_cast<size_t>(g) * a.beams + w) * chunks;
+        float m = -INFINITY, s = 0.f;
+        for (int c = lane; c < chunks; c += 32) m = fmaxf(m, __ldcg(st + c).x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
+        for (int c = lane; c < chunks; c += 32) {
+            const float2 v = __ldcg(st + c);
+            s += v.y * expf(v.x == -INFINITY ? (m == -INFINITY ? 0.f : -INFINITY) : v.x - m);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+        if (lane == 0) {
+            sm.lse[w] = m + logf(s);
+            sm.score[w] = a.scores[static_cast<size_t>(g) * a.beams + w];
+        }
+    }
+    __syncthreads();
+    const int n_lists = a.beams * chunks;
+    const uint64_t* keys = lists + static_cast<size_t>(g) * n_lists * a.keep;
+    auto read = [&](int l, int k) {  // candidate k of list l
+        Best b;
+        b.key = __ldcg(keys + static_cast<size_t>(l) * a.keep + k);
+        b.row = l / chunks;
+        const float v = sm.score[b.row] + (candidate_value(b.key) - sm.lse[b.row]);
+        b.bits = b.key == 0 ? 0u : float_order_key(isnan(v) ? -INFINITY : v + 0.f);
+        return b;
+    };
+    // 512 walkers: with fewer lists, several take a list's candidates in turn. The first candidates of each are the samples.
+    const int across = min(n_lists, kSamples), step = kSamples / across;
+    for (int v = threadIdx.x; v < kSamples; v += THREADS) {
+        const int k0 = v / across;
+        uint32_t top = 0;
+        if (k0 < step && k0 < a.keep) {
+            for (int l = v % across; l < n_lists; l += across) top = max(top, read(l, k0).bits);
+        }
+        sm.samples[v] = top;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t b = bound_of(sm.samples, a.keep);
+        if (lane == 0) sm.bound = max(b, 1u);
+    }
+    __syncthreads();
+    const uint32_t bound = sm.bound;
+    auto each = [&](auto&& take) {  // every candidate from the bound on
+        for (int v = threadIdx.x; v < kSamples; v += THREADS) {
+            const int k0 = v / across;
+            if (k0 >= step) break;
+            for (int l = v % across; l < n_lists; l += across) {
+                for (int k = k0; k < a.keep; k += step) {
+                    const Best b = read(l, k);
+                    if (b.bits < bound) break;  // lists descend
+                    take(b);
+                }
+            }
+        }
+    };
+    each([&](const Best& b) {
+        const int p = atomicAdd(&sm.count, 1);
+        if (p < kGroupList) sm.list[p] = b;
+    });
+    __syncthreads();
+    auto write = [&](int k, const Best& b) {
+        const size_t o = static_cast<size_t>(g) * a.keep + k;
+        a.out_scores[o] = float_from_order_key(b.bits);
+        a.out_parents[o] = g * a.beams + b.row;
+        a.out_tokens[o] = candidate_index(b.key);
+    };
+    const int count = sm.count;
+    if (count <= kGroupList) {
+        for (int c = threadIdx.x; c < count; c += THREADS) {
+            const Best b = sm.list[c];
+            int rank = 0;
+            for (int i = 0; i < count; ++i) rank += better(sm.list[i], b);
+            if (rank < a.keep) write(rank, b);
+        }
+        return;
+    }
+    // Too many ties to count: one winner after the other.
+    Best last{kAll, -1, ~0ull};
+    for (int k = 0; k < a.keep; ++k) {
+        Best best{0, kMaxBeams, 0};
+        each([&](const Best& b) {
+            if (better(last, b) && better(b, best)) best = b;
+        });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const Best b{__shfl_xor_sync(kAll, best.bits, o), __shfl_xor_sync(kAll, best.row, o), __shfl_xor_sync(kAll, best.key, o)};
+            if (better(b, best)) best = b;
+        }
+        __syncthreads();
+        if (lane == 0) sm.best[warp] = best;
+        __syncthreads();
+        best = sm.best[0];
+        for (int w = 1; w < THREADS / 32; ++w)
+            if (better(sm.best[w], best)) best = sm.best[w];
+        if (threadIdx.x == 0) write(k, best);
+        last = best;
+    }
+}
+
 // 2^x to 22 bits, which a sum of thousands of them averages out; exp(x) = 2^(x log2(e)).
 __device__ __forceinline__ float exp_fast(float x) {
     float y;
@@ -72,27 +199,18 @@ __device__ __forceinline__ float exp_fast(float x) {
     return y;
 }
 
+struct ChunkRoom {
+    uint64_t list[kList];
+    float m[kThreads / 32], s[kThreads / 32];
+    uint32_t samples[kSamples], bound;
+    int n[kThreads / 32], count;
+};
+
+// The sorted list and the sums of one chunk of a row that goes on.
 template <typename X>
-__global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const __grid_constant__ cudallm_beam_args a, uint64_t* lists, float2* stats, int chunks,
-                                                              bool wide) {
-    __shared__ uint64_t list[kList];
-    __shared__ float sm_m[kThreads / 32], sm_s[kThreads / 32];
-    __shared__ uint32_t samples[2 * kThreads], sm_bound;
-    __shared__ int sm_n[kThreads / 32], sm_count;
-    static_assert(2 * kThreads == 512, "bound_of takes 512");
-    grid_dep_launch();
-    const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const size_t place = blockIdx.x;
-    uint64_t* out = lists + place * a.keep;
-    if (a.finished != nullptr && a.finished[row] != 0) {
-        // 0 at eos, then -inf from the lowest token on; the other chunks of the row have nothing.
-        for (int k = threadIdx.x; k < a.keep; k += kThreads) {
-            const int t = k == 0 ? a.eos : k - 1 + (k - 1 >= a.eos ? 1 : 0);
-            out[k] = chunk == 0 && t < a.vocab ? candidate_key(k == 0 ? 0.f : -INFINITY, t) : 0;
-        }
-        if (threadIdx.x == 0) stats[place] = chunk == 0 ? make_float2(0.f, 1.f) : make_float2(-INFINITY, 0.f);
-        return;
-    }
+__device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, int chunk, bool wide, uint64_t* out, float2* stat, ChunkRoom& sm) {
+    static_assert(2 * kThreads == kSamples, "two sm.samples of every thread");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const X* x = static_cast<const X*>(a.logits) + row * a.row_stride;
     constexpr int kVec = 16 / sizeof(X);
     const int c0 = chunk * kChunk, n = min(kChunk, a.vocab - c0);
@@ -138,36 +256,36 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const __grid_const
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
     if (lane == 0) {
-        sm_m[warp] = m;
-        sm_s[warp] = s;
+        sm.m[warp] = m;
+        sm.s[warp] = s;
     }
-    samples[threadIdx.x] = top[0];
-    samples[kThreads + threadIdx.x] = top[1];
+    sm.samples[threadIdx.x] = top[0];
+    sm.samples[kThreads + threadIdx.x] = top[1];
     __syncthreads();
     if (warp == 0) {
-        const uint32_t b = bound_of(samples, a.keep);
+        const uint32_t b = bound_of(sm.samples, a.keep);
         if (lane == 0) {
-            sm_bound = max(b, 1u);  // places without a logit are never taken
-            sm_count = 0;
+            sm.bound = max(b, 1u);  // places without a logit are never taken
+            sm.count = 0;
         }
     }
     if (threadIdx.x == 32) {
         float mm = -INFINITY, ss = 0.f;
-        for (int w = 0; w < kThreads / 32; ++w) mm = fmaxf(mm, sm_m[w]);
-        for (int w = 0; w < kThreads / 32; ++w) ss += sm_s[w] * expf(sm_m[w] == -INFINITY ? (mm == -INFINITY ? 0.f : -INFINITY) : sm_m[w] - mm);
-        stats[place] = make_float2(mm, ss);
+        for (int w = 0; w < kThreads / 32; ++w) mm = fmaxf(mm, sm.m[w]);
+        for (int w = 0; w < kThreads / 32; ++w) ss += sm.s[w] * expf(sm.m[w] == -INFINITY ? (mm == -INFINITY ? 0.f : -INFINITY) : sm.m[w] - mm);
+        *stat = make_float2(mm, ss);
     }
     __syncthreads();
-    uint32_t bound = sm_bound;
+    uint32_t bound = sm.bound;
     auto push = [&](int j) {
-        const int p = atomicAdd(&sm_count, 1);
-        if (p < kList) list[p] = static_cast<uint64_t>(bits[j]) << 32 | static_cast<uint32_t>(~(c0 + at(j)));
+        const int p = atomicAdd(&sm.count, 1);
+        if (p < kList) sm.list[p] = static_cast<uint64_t>(bits[j]) << 32 | static_cast<uint32_t>(~(c0 + at(j)));
     };
 #pragma unroll
     for (int j = 0; j < kEach; ++j)
         if (bits[j] >= bound) push(j);
     __syncthreads();
-    if (sm_count > kList) {
+    if (sm.count > kList) {
         // Too many ties to list: the keep-th value, then how far its ties go.
         bound = 0;
 #pragma unroll 1
@@ -176,12 +294,12 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const __grid_const
             int above = 0;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) above += bits[j] >= test;
-            if (block_sum<kThreads>(above, sm_n) >= a.keep) bound = test;
+            if (block_sum<kThreads>(above, sm.n) >= a.keep) bound = test;
         }
         int above = 0;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) above += bits[j] > bound;
-        const int ties = a.keep - block_sum<kThreads>(above, sm_n);  // wanted: 1 or more
+        const int ties = a.keep - block_sum<kThreads>(above, sm.n);  // wanted: 1 or more
         uint32_t last = 0;  // the largest place with fewer ties before it
 #pragma unroll 1
         for (int bit = 11; bit >= 0; --bit) {
@@ -189,142 +307,66 @@ __global__ void __launch_bounds__(kThreads) beam_chunk_kernel(const __grid_const
             above = 0;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) above += bits[j] == bound && at(j) < static_cast<int>(test);
-            if (block_sum<kThreads>(above, sm_n) < ties) last = test;
+            if (block_sum<kThreads>(above, sm.n) < ties) last = test;
         }
-        if (threadIdx.x == 0) sm_count = 0;
+        if (threadIdx.x == 0) sm.count = 0;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
             if (bits[j] > bound || (bits[j] == bound && static_cast<uint32_t>(at(j)) <= last)) push(j);
     }
     __syncthreads();
-    const int count = min(sm_count, kList);
+    const int count = min(sm.count, kList);
     if (threadIdx.x < count) {
-        const uint64_t key = list[threadIdx.x];
+        const uint64_t key = sm.list[threadIdx.x];
         int rank = 0;
-        for (int i = 0; i < count; ++i) rank += list[i] > key;
+        for (int i = 0; i < count; ++i) rank += sm.list[i] > key;
         if (rank < a.keep) out[rank] = key;
     }
     for (int k = count + threadIdx.x; k < a.keep; k += kThreads) out[k] = 0;
 }
 
-struct Best {
-    uint32_t bits;  // of the candidate
-    int row;        // beam in the group
-    uint64_t key;   // logit and token
-};
-__device__ __forceinline__ bool better(const Best& a, const Best& b) {
-    return a.bits != b.bits ? a.bits > b.bits : a.row != b.row ? a.row < b.row : a.key > b.key;
+// Block = chunk of a row. With `counts` (one zero for each group), the last block of a group to finish selects its best.
+template <typename X>
+__global__ void __launch_bounds__(kThreads, 5) beam_chunk_kernel(const __grid_constant__ cudallm_beam_args a, uint64_t* lists, float2* stats, int chunks, bool wide,
+                                                                 unsigned* counts) {
+    __shared__ union {
+        ChunkRoom chunk;
+        GroupRoom<kThreads> group;
+    } room;
+    __shared__ bool last;
+    grid_dep_launch();
+    const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
+    const size_t place = blockIdx.x;
+    uint64_t* out = lists + place * a.keep;
+    if (a.finished != nullptr && a.finished[row] != 0) {
+        // 0 at eos, then -inf from the lowest token on; the other chunks of the row have nothing.
+        for (int k = threadIdx.x; k < a.keep; k += kThreads) {
+            const int t = k == 0 ? a.eos : k - 1 + (k - 1 >= a.eos ? 1 : 0);
+            out[k] = chunk == 0 && t < a.vocab ? candidate_key(k == 0 ? 0.f : -INFINITY, t) : 0;
+        }
+        if (threadIdx.x == 0) stats[place] = chunk == 0 ? make_float2(0.f, 1.f) : make_float2(-INFINITY, 0.f);
+    } else {
+        list_chunk<X>(a, row, chunk, wide, out, stats + place, room.chunk);
+    }
+    if (counts == nullptr) return;
+    __syncthreads();
+    const int g = row / a.beams;
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = atomicAdd(counts + g, 1u) == static_cast<unsigned>(a.beams * chunks - 1);
+        if (last) counts[g] = 0u;
+        __threadfence();
+    }
+    __syncthreads();
+    if (last) select_group<kThreads>(a, lists, stats, chunks, g, room.group);
 }
 
 __global__ void __launch_bounds__(kGroupThreads) beam_group_kernel(const __grid_constant__ cudallm_beam_args a, const uint64_t* lists, const float2* stats,
                                                                    int chunks) {
-    __shared__ float lse[kMaxBeams], score[kMaxBeams];
-    __shared__ Best list[kGroupList];
-    __shared__ uint32_t samples[kGroupThreads], sm_bound;
-    __shared__ int sm_count;
-    const int g = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) sm_count = 0;
+    __shared__ GroupRoom<kGroupThreads> room;
     grid_dep_wait();
-    for (int w = warp; w < a.beams; w += kGroupThreads / 32) {
-        const float2* st = stats + (static_cast<size_t>(g) * a.beams + w) * chunks;
-        float m = -INFINITY, s = 0.f;
-        for (int c = lane; c < chunks; c += 32) m = fmaxf(m, __ldcg(st + c).x);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
-        for (int c = lane; c < chunks; c += 32) {
-            const float2 v = __ldcg(st + c);
-            s += v.y * expf(v.x == -INFINITY ? (m == -INFINITY ? 0.f : -INFINITY) : v.x - m);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
-        if (lane == 0) {
-            lse[w] = m + logf(s);
-            score[w] = a.scores[static_cast<size_t>(g) * a.beams + w];
-        }
-    }
-    __syncthreads();
-    const int n_lists = a.beams * chunks;
-    const uint64_t* keys = lists + static_cast<size_t>(g) * n_lists * a.keep;
-    auto read = [&](int l, int k) {  // candidate k of list l
-        Best b;
-        b.key = __ldcg(keys + static_cast<size_t>(l) * a.keep + k);
-        b.row = l / chunks;
-        const float v = score[b.row] + (candidate_value(b.key) - lse[b.row]);
-        b.bits = b.key == 0 ? 0u : float_order_key(isnan(v) ? -INFINITY : v + 0.f);
-        return b;
-    };
-    // With fewer lists than threads, several threads take a list's candidates in turn; the first of each thread are the samples.
-    const int across = min(n_lists, kGroupThreads), step = kGroupThreads / across;
-    const int l0 = threadIdx.x % across, k0 = threadIdx.x / across;
-    const bool works = k0 < step && k0 < a.keep;
-    uint32_t top = 0;
-    if (works) {
-        for (int l = l0; l < n_lists; l += across) top = max(top, read(l, k0).bits);
-    }
-    samples[threadIdx.x] = top;
-    __syncthreads();
-    if (warp == 0) {
-        const uint32_t b = bound_of(samples, a.keep);
-        if (lane == 0) sm_bound = max(b, 1u);
-    }
-    __syncthreads();
-    const uint32_t bound = sm_bound;
-    if (works) {
-        for (int l = l0; l < n_lists; l += across) {
-            for (int k = k0; k < a.keep; k += step) {
-                const Best b = read(l, k);
-                if (b.bits < bound) break;  // lists descend
-                const int p = atomicAdd(&sm_count, 1);
-                if (p < kGroupList) list[p] = b;
-            }
-        }
-    }
-    __syncthreads();
-    const int count = sm_count;
-    auto write = [&](int k, const Best& b) {
-        const size_t o = static_cast<size_t>(g) * a.keep + k;
-        a.out_scores[o] = float_from_order_key(b.bits);
-        a.out_parents[o] = g * a.beams + b.row;
-        a.out_tokens[o] = candidate_index(b.key);
-    };
-    if (count <= kGroupList) {
-        if (threadIdx.x < count) {
-            const Best b = list[threadIdx.x];
-            int rank = 0;
-            for (int i = 0; i < count; ++i) rank += better(list[i], b);
-            if (rank < a.keep) write(rank, b);
-        }
-        return;
-    }
-    // Too many ties to count: one winner after the other.
-    __shared__ Best sm_best[kGroupThreads / 32];
-    Best last{kAll, -1, ~0ull};
-    for (int k = 0; k < a.keep; ++k) {
-        Best best{0, kMaxBeams, 0};
-        if (works) {
-            for (int l = l0; l < n_lists; l += across) {
-                for (int i = k0; i < a.keep; i += step) {
-                    const Best b = read(l, i);
-                    if (b.bits < bound) break;
-                    if (better(last, b) && better(b, best)) best = b;
-                }
-            }
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const Best b{__shfl_xor_sync(kAll, best.bits, o), __shfl_xor_sync(kAll, best.row, o), __shfl_xor_sync(kAll, best.key, o)};
-            if (better(b, best)) best = b;
-        }
-        __syncthreads();
-        if (lane == 0) sm_best[warp] = best;
-        __syncthreads();
-        best = sm_best[0];
-        for (int w = 1; w < kGroupThreads / 32; ++w)
-            if (better(sm_best[w], best)) best = sm_best[w];
-        if (threadIdx.x == 0) write(k, best);
-        last = best;
-    }
+    select_group<kGroupThreads>(a, lists, stats, chunks, blockIdx.x, room);
 }
 
 int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
@@ -333,20 +375,23 @@ int chunks_of(int vocab) { return (vocab + kChunk - 1) / kChunk; }
 
 size_t beam_workspace_bytes(int rows, int vocab, int keep) {
     if (rows < 0 || rows > kMaxPageRows || vocab < 1 || vocab > kMaxVocab || keep < 1 || keep > kMaxKeep) return 0;
-    return 256 + (sizeof(float2) + sizeof(uint64_t) * keep) * static_cast<size_t>(rows) * chunks_of(vocab);
+    return CUDALLM_BEAM_COUNTER_BYTES + (sizeof(float2) + sizeof(uint64_t) * keep) * static_cast<size_t>(rows) * chunks_of(vocab);
 }
 
 void launch_beam_select(const cudallm_beam_args& a, cudaStream_t stream) {
     if (a.n_groups == 0) return;
     const int rows = a.n_groups * a.beams, chunks = chunks_of(a.vocab);
-    auto* stats = static_cast<float2*>(a.workspace);
+    const bool one = static_cast<long long>(rows) * chunks <= kOneLaunch && a.n_groups <= static_cast<int>(CUDALLM_BEAM_COUNTER_BYTES / 4);
+    auto* counts = one ? static_cast<unsigned*>(a.workspace) : nullptr;
+    auto* stats = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + CUDALLM_BEAM_COUNTER_BYTES);
     auto* lists = reinterpret_cast<uint64_t*>(stats + static_cast<size_t>(rows) * chunks);
     const size_t es = a.x_dtype == CUDALLM_X_FP32 ? 4 : 2;
     const bool wide = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (rows == 1 || a.row_stride * es % 16 == 0);
     auto* kernel = a.x_dtype == CUDALLM_X_FP32   ? beam_chunk_kernel<float>
                    : a.x_dtype == CUDALLM_X_FP16 ? beam_chunk_kernel<__half>
                                                  : beam_chunk_kernel<__nv_bfloat16>;
-    launch_kernel(kernel, dim3(rows * chunks), dim3(kThreads), 0, stream, false, a, lists, stats, chunks, wide);
+    launch_kernel(kernel, dim3(rows * chunks), dim3(kThreads), 0, stream, false, a, lists, stats, chunks, wide, counts);
+    if (counts != nullptr) return;
     launch_kernel(beam_group_kernel, dim3(a.n_groups), dim3(kGroupThreads), 0, stream, true, a, static_cast<const uint64_t*>(lists),
                   static_cast<const float2*>(stats), chunks);
 }

@@ -38,6 +38,7 @@ except ImportError:
 _X = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _KV = {torch.float16: 0, torch.bfloat16: 1}
 _INVALID_ARG = 1
+_BEAM_COUNTERS = 16384  # CUDALLM_BEAM_COUNTER_BYTES
 
 
 def _refuse(message: str):
@@ -74,16 +75,22 @@ def _beam_args():
 class _Workspaces:
     """A workspace for each of a device's streams (calls on different streams may overlap)."""
 
-    def __init__(self, device: torch.device):
-        self.device = device
+    def __init__(self, device: torch.device, counters: int = 0):
+        self.device, self.counters = device, counters  # leading bytes that start at zero
         self.by_stream: dict[int, torch.Tensor] = {}
+
+    def _new(self, size: int) -> torch.Tensor:
+        w = torch.empty(size, dtype=torch.uint8, device=self.device)
+        if self.counters:
+            w[:self.counters].zero_()
+        return w
 
     def get(self, stream: int, size: int) -> torch.Tensor:
         if torch.cuda.is_current_stream_capturing():  # the graph's own, which later calls must not replace
-            return torch.empty(size, dtype=torch.uint8, device=self.device)
+            return self._new(size)
         w = self.by_stream.get(stream)
         if w is None or w.numel() < size:
-            w = self.by_stream[stream] = torch.empty(size, dtype=torch.uint8, device=self.device)
+            w = self.by_stream[stream] = self._new(size)
         return w
 
 
@@ -396,7 +403,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     stream = _stream_of(index)
     spaces = _shared.get(index)
     if spaces is None:
-        spaces = _shared[index] = _Workspaces(dev)
+        spaces = _shared[index] = _Workspaces(dev, _BEAM_COUNTERS)
     w = spaces.get(stream, size(rows, vocab, keep))
     a.workspace, a.workspace_bytes = w.data_ptr(), w.numel()
     if torch.cuda.current_device() == index:

@@ -250,8 +250,11 @@ int cudallm_attention_noalloc(const float* q, const unsigned short* k_cache, con
  * What the host cannot see (lengths, tables, positions, parents) is bounded inside the kernels as stated below,
  * so no content of those arrays leads to an access outside of the caller's buffers.
  *
- * Workspaces: `workspace` points to at least cudallm_*_workspace_bytes() bytes, 256-byte aligned; its contents do not matter. One may serve
- * all of these calls, one after the other on one stream; calls that may overlap (other streams) need their own. */
+ * Workspaces: `workspace` points to at least cudallm_*_workspace_bytes() bytes, 256-byte aligned; its contents do not matter (but for
+ * cudallm_beam_select's, see there). One may serve the cudallm_paged_* calls one after the other on one stream; calls that may overlap (other
+ * streams) need their own. */
+
+#define CUDALLM_BEAM_COUNTER_BYTES 16384
 
 #define CUDALLM_X_FP32 0
 #define CUDALLM_X_FP16 1
@@ -394,7 +397,8 @@ typedef struct {
 
 int cudallm_beam_select(const cudallm_beam_args* args, void* stream);
 /* Workspace of cudallm_beam_select for up to `rows` = n_groups * beams rows of up to vocab logits; 0 for sizes that
- * the call refuses. */
+ * the call refuses. Unlike the others' it must have its first CUDALLM_BEAM_COUNTER_BYTES bytes zero before the first call with
+ * it; every call leaves them zero. So it is not shared with the calls above. */
 unsigned long long cudallm_beam_workspace_bytes(int rows, int vocab, int keep);
 
 #ifdef __cplusplus

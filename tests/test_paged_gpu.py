@@ -495,6 +495,12 @@ def test_beam_sizes(x, groups, beams, keep, vocab):
     _check_beam(logits, scores, keep)
 
 
+def test_beam_many_groups():
+    """More groups than the single launch has counters for."""
+    logits = torch.randn((5000 * 2, 45), device="cuda", dtype=BF16)
+    _check_beam(logits, np.random.default_rng(0).normal(-4, 1, (5000, 2)), 3)
+
+
 @pytest.mark.parametrize("vocab", [5, 900, 70001])
 def test_beam_ties_go_to_the_lower_row_then_token(vocab):
     keep = 9

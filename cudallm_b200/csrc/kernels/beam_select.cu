@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, 5) beam_chunk_kernel(const __grid_co
         GroupRoom<kThreads> group;
     } room;
     __shared__ bool last;
+    grid_dep_wait();
     grid_dep_launch();
     const int row = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
     const size_t place = blockIdx.x;
@@ -390,7 +391,7 @@ void launch_beam_select(const cudallm_beam_args& a, cudaStream_t stream) {
     auto* kernel = a.x_dtype == CUDALLM_X_FP32   ? beam_chunk_kernel<float>
                    : a.x_dtype == CUDALLM_X_FP16 ? beam_chunk_kernel<__half>
                                                  : beam_chunk_kernel<__nv_bfloat16>;
-    launch_kernel(kernel, dim3(rows * chunks), dim3(kThreads), 0, stream, false, a, lists, stats, chunks, wide, counts);
+    launch_kernel(kernel, dim3(rows * chunks), dim3(kThreads), 0, stream, true, a, lists, stats, chunks, wide, counts);
     if (counts != nullptr) return;
     launch_kernel(beam_group_kernel, dim3(a.n_groups), dim3(kGroupThreads), 0, stream, true, a, static_cast<const uint64_t*>(lists),
                   static_cast<const float2*>(stats), chunks);

@@ -15,6 +15,7 @@
 #include "kernels/launch.cuh"
 #include "kernels/paged.h"
 #include "kernels/paged_common.cuh"
+#include "kernels/ptx.cuh"
 
 namespace cudallm {
 
@@ -171,6 +172,8 @@ __global__ void __launch_bounds__(kThreads, few_registers<X, L> ? 4 : 5) append_
     __shared__ __align__(16) float cos[kTokens][128], sin[kTokens][128];
     __shared__ long long slots[kTokens];  // where the token's keys go; -1: nowhere, -2: padding
     const cudallm_append_args& a = p.a;
+    grid_dep_wait();
+    grid_dep_launch();
     const int first = blockIdx.x * p.tokens, tokens = min(p.tokens, a.n_tokens - first);
     if (threadIdx.x < tokens) {
         const int i = first + threadIdx.x, pos = a.positions[i], row = a.rows != nullptr ? a.rows[i] : i;
@@ -295,7 +298,7 @@ void launch_for(Params& p, cudaStream_t stream) {
     auto kernel = !wide           ? append_kernel<X, KV, Layout::kSingle>
                   : a.interleaved ? append_kernel<X, KV, Layout::kInterleaved>
                                   : append_kernel<X, KV, Layout::kHalves>;
-    launch_kernel(kernel, dim3(blocks, spread), dim3(kThreads), 0, stream, false, p);
+    launch_kernel(kernel, dim3(blocks, spread), dim3(kThreads), 0, stream, true, p);
 }
 
 template <typename X>

@@ -245,6 +245,7 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
     unsigned* before = reinterpret_cast<unsigned*>(smem + S::kFixed);                // [n_seq + 1]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t4 = lane & 3, hd = p.head_dim;
+    grid_dep_wait();
     if (threadIdx.x == 0) p.endings[blockIdx.x].n = 0;
     grid_dep_launch();  // the join's blocks may take the places that this kernel's leave
 
@@ -817,7 +818,7 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
         const size_t smem = S::kFixed + 4 * (static_cast<size_t>(p.n_seq) + 1);
         const long long most = std::max<long long>(1, (row_tiles + kUnit - 1) / kUnit * p.n_seq + p.items * static_cast<long long>(p.n_seq));
         const int grid = static_cast<int>(std::min<long long>(std::min(kMaxCtas, num_sms() * std::min(S::kCtas, static_cast<int>(228 * 1024 / (smem + 1024)))), most));
-        launch_kernel(kernel, dim3(grid), dim3(kThreads), smem, stream, false, p);
+        launch_kernel(kernel, dim3(grid), dim3(kThreads), smem, stream, true, p);
         // Items of up to kUnit tiles are cut only where equal shares cut them, which takes more tiles than there are CTAs x kUnit.
         const bool can_cut = (cap + S::kTile - 1) / S::kTile > kUnit || static_cast<long long>(p.n_seq) * p.items > grid;
         if (can_cut) launch_kernel(join_kernel<X, HD>, dim3(grid, std::min(p.group, S::kHeads)), dim3(32 * kJoinWarps), 0, stream, true, p);

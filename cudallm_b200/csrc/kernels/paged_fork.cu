@@ -291,6 +291,7 @@ __device__ __forceinline__ void fork_copies(const cudallm_pages& pg, const ForkP
 __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
                                                                  bool wide) {
     extern __shared__ int shared_counters[];
+    grid_dep_wait();
     grid_dep_launch();
     if (blockIdx.x > 0) {
         for (int p = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; p < pg.n_pages; p += (gridDim.x - 1) * kPlanThreads) a.refs_out[p] = a.refs[p];
@@ -317,6 +318,8 @@ __global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constan
                                                             bool wide) {
     extern __shared__ __align__(16) char room[];
     const ForkPlan s = fork_plan(room, rows, kOneFound);
+    grid_dep_wait();
+    grid_dep_launch();
     if (blockIdx.x == 0) {
         for (int p = threadIdx.x; p < pg.n_pages; p += kPlanThreads) a.refs_out[p] = a.refs[p];
     }
@@ -408,6 +411,7 @@ __device__ __forceinline__ void move_compact(const cudallm_pages& pg, const cuda
 
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
                                                                     bool wide) {
+    grid_dep_wait();
     grid_dep_launch();
     plan_compact(pg, a, s, wide);
 }
@@ -422,6 +426,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(const __grid_cons
                                                                bool wide) {
     extern __shared__ __align__(16) char room[];
     const CompactPlan s = compact_plan(room, pg.n_pages);
+    grid_dep_wait();
+    grid_dep_launch();
     plan_compact(pg, a, s, wide);
     move_compact<2>(pg, a, s, by_row, static_cast<long long>(blockIdx.x) * kPlanThreads + threadIdx.x, static_cast<long long>(gridDim.x) * kPlanThreads);
 }
@@ -445,13 +451,13 @@ void launch_paged_fork(const cudallm_pages& pg, const cudallm_fork_args& a, cuda
         heads <= kOneHeads) {
         constexpr int kWarps = kPlanThreads / 32;
         const int blocks = 1 + static_cast<int>(std::min<long long>(sms - 1, std::max<long long>(1, (heads + kWarps - 1) / kWarps)));
-        launch_kernel(fork_kernel, dim3(blocks), dim3(kPlanThreads), fork_plan_bytes(rows, kOneFound), stream, false, pg, a, rows, by_row, wide);
+        launch_kernel(fork_kernel, dim3(blocks), dim3(kPlanThreads), fork_plan_bytes(rows, kOneFound), stream, true, pg, a, rows, by_row, wide);
         return;
     }
     const ForkPlan s = fork_plan(a.workspace, rows, pg.n_pages);
     const int copiers = std::min(sms, (pg.n_pages + kPlanThreads - 1) / kPlanThreads);  // of the references
     const size_t smem = a.n_rows <= kSharedRows ? 8 * static_cast<size_t>(a.n_rows) : 0;
-    launch_kernel(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), smem, stream, false, pg, a, s, wide);
+    launch_kernel(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), smem, stream, true, pg, a, s, wide);
     if (rows == 0) return;
     const int movers = static_cast<int>(std::min<long long>(8LL * sms, (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
     const long long entries = static_cast<long long>(rows) * a.table_width;
@@ -468,11 +474,11 @@ void launch_paged_compact(const cudallm_pages& pg, const cudallm_compact_args& a
         static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
         allow_shared(compact_kernel, static_cast<int>(compact_plan_bytes(kOnePages)), allowed);
         const long long most = 1 + (heads + kPlanThreads / 32 - 1) / (kPlanThreads / 32);
-        launch_kernel(compact_kernel, dim3(static_cast<int>(std::min<long long>(num_sms(), most))), dim3(kPlanThreads), smem, stream, false, pg, a, by_row, wide);
+        launch_kernel(compact_kernel, dim3(static_cast<int>(std::min<long long>(num_sms(), most))), dim3(kPlanThreads), smem, stream, true, pg, a, by_row, wide);
         return;
     }
     const CompactPlan s = compact_plan(a.workspace, pg.n_pages);
-    launch_kernel(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, false, pg, a, s, wide);
+    launch_kernel(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, true, pg, a, s, wide);
     const int blocks = static_cast<int>(std::min<long long>(8LL * num_sms(), 1 + (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
     launch_kernel(compact_move_kernel, dim3(blocks), dim3(kMoveThreads), 0, stream, true, pg, a, s, by_row);
 }

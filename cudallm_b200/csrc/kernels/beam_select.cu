@@ -6,9 +6,8 @@
 // only ones that can be among the group's.
 //
 // chunk stage: one block per 4096 logits, which stay in registers (one read of the logits, what bounds the operator at
-//   many rows). It leaves their maximum, their sum of exponentials and the sorted keys of their `keep` best. A lower
-//   bound of the keep-th best is the keep-th largest of the maxima of 512 pieces; the few logits above it are ranked by
-//   counting. Where more than 256 are above it (ties, a masked vocabulary) the keep-th key itself is
+//   many rows). It leaves their maximum, their sum of exponentials and the sorted keys of their `keep` best. The maxima of 512
+//   pieces give a lower bound of the keep-th best; the few logits above it are ranked by counting. Where more than 256 are above it (ties, a masked vocabulary) the keep-th key itself is
 //   searched bit by bit over value and token.
 // group stage: joins the rows' sums and ranks the lists' candidates in the same way. Up to 256 chunks the last block of a
 //   group to finish does it; with more, a block for each group in a second launch, in place when the chunks are done (4 rows x
@@ -37,6 +36,32 @@ constexpr unsigned kAll = 0xffffffffu;
 
 // Rank bits of a logit: not a number counts as -inf, -0 as 0.
 __device__ __forceinline__ uint32_t logit_bits(float x) { return float_order_key(isnan(x) ? -INFINITY : x + 0.f); }
+
+// The first 16 bits of the r-th largest of the values a, b of a warp's lanes (0 = none, or fewer than r of them): a lower bound of it.
+__device__ __forceinline__ uint32_t warp_bound(uint32_t a, uint32_t b, int r) {
+    uint32_t bound = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t test = bound | 1u << bit;
+        if (__popc(__ballot_sync(kAll, a >= test)) + __popc(__ballot_sync(kAll, b >= test)) >= r) bound = test;
+    }
+    return bound;
+}
+
+// A lower bound of the keep-th largest of a block's values, of which every thread brings two samples: where each of `warps` warps has r =
+// keep / warps samples from its bound on, there are `keep` from the smallest of those bounds on. `sm` has a place for each warp;
+// a barrier inside. At least 1, as values are.
+template <int THREADS>
+__device__ __forceinline__ uint32_t block_bound(uint32_t a, uint32_t b, int keep, int warps, uint32_t* sm) {
+    warps = max(warps, 1);
+    const uint32_t mine = warp_bound(a, b, (keep + warps - 1) / warps);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = static_cast<int>(threadIdx.x >> 5) < warps ? mine : kAll;
+    __syncthreads();
+    uint32_t bound = kAll;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) bound = min(bound, sm[w]);
+    return max(bound, 1u);
+}
 
 // The first 16 bits of the keep-th largest of 512 values in shared memory (0 = none, or fewer than keep): a lower bound of it. One warp.
 __device__ __forceinline__ uint32_t bound_of(const uint32_t* samples, int keep) {
@@ -129,7 +154,7 @@ __device__ void select_group(const cudallm_beam_args& a, const uint64_t* lists, 
         sm.samples[v] = top;
     }
     __syncthreads();
-    if (warp == 0) {
+    if (warp == 0) {  // rows differ by their scores, so that no part of the lists says much about the others
         const uint32_t b = bound_of(sm.samples, a.keep);
         if (lane == 0) sm.bound = max(b, 1u);
     }
@@ -202,14 +227,13 @@ __device__ __forceinline__ float exp_fast(float x) {
 struct ChunkRoom {
     uint64_t list[kList];
     float m[kThreads / 32], s[kThreads / 32];
-    uint32_t samples[kSamples], bound;
+    uint32_t bounds[kThreads / 32];
     int n[kThreads / 32], count;
 };
 
 // The sorted list and the sums of one chunk of a row that goes on.
 template <typename X>
 __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, int chunk, bool wide, uint64_t* out, float2* stat, ChunkRoom& sm) {
-    static_assert(2 * kThreads == kSamples, "two sm.samples of every thread");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const X* x = static_cast<const X*>(a.logits) + row * a.row_stride;
     constexpr int kVec = 16 / sizeof(X);
@@ -259,24 +283,16 @@ __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, 
         sm.m[warp] = m;
         sm.s[warp] = s;
     }
-    sm.samples[threadIdx.x] = top[0];
-    sm.samples[kThreads + threadIdx.x] = top[1];
-    __syncthreads();
-    if (warp == 0) {
-        const uint32_t b = bound_of(sm.samples, a.keep);
-        if (lane == 0) {
-            sm.bound = max(b, 1u);  // places without a logit are never taken
-            sm.count = 0;
-        }
-    }
+    if (threadIdx.x == 0) sm.count = 0;
+    // Threads with two logits or more have two samples.
+    const int sampled = wide ? n / kVec : max(0, n - kThreads);
+    uint32_t bound = block_bound<kThreads>(top[0], top[1], a.keep, min(sampled, kThreads) / 32, sm.bounds);
     if (threadIdx.x == 32) {
         float mm = -INFINITY, ss = 0.f;
         for (int w = 0; w < kThreads / 32; ++w) mm = fmaxf(mm, sm.m[w]);
         for (int w = 0; w < kThreads / 32; ++w) ss += sm.s[w] * expf(sm.m[w] == -INFINITY ? (mm == -INFINITY ? 0.f : -INFINITY) : sm.m[w] - mm);
         *stat = make_float2(mm, ss);
     }
-    __syncthreads();
-    uint32_t bound = sm.bound;
     auto push = [&](int j) {
         const int p = atomicAdd(&sm.count, 1);
         if (p < kList) sm.list[p] = static_cast<uint64_t>(bits[j]) << 32 | static_cast<uint32_t>(~(c0 + at(j)));

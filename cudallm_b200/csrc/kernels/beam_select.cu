@@ -217,10 +217,10 @@ __device__ void select_group(const cudallm_beam_args& a, const uint64_t* lists, 
     }
 }
 
-// 2^x to 22 bits, which a sum of thousands of them averages out; exp(x) = 2^(x log2(e)).
-__device__ __forceinline__ float exp_fast(float x) {
+// 2^x to 22 bits, which a sum of thousands of them averages out.
+__device__ __forceinline__ float exp2_fast(float x) {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -262,21 +262,19 @@ __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, 
 #pragma unroll
         for (int j = 0; j < kEach; ++j) v[j] = at(j) < n ? as_float(x[c0 + at(j)]) : -INFINITY;
     }
-    // Rank bits; 0 where there is no logit (every logit's are above 0).
-    uint32_t bits[kEach], top[2] = {0, 0};
-    float m = -INFINITY;
+    auto inside = [&](int j) { return n == kChunk || at(j) < n; };
+    float top[2] = {-INFINITY, -INFINITY};  // what is not a number is left out, as -inf would be
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        bits[j] = at(j) < n ? logit_bits(v[j]) : 0u;
-        top[j & 1] = max(top[j & 1], bits[j]);
-        m = fmaxf(m, v[j]);
-    }
+    for (int j = 0; j < kEach; ++j) top[j & 1] = fmaxf(top[j & 1], v[j]);
+    float m = fmaxf(top[0], top[1]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
     const float ref = m == -INFINITY ? 0.f : m;
+    constexpr float kLog2e = 1.4426950408889634f;
+    const float shift = -ref * kLog2e;
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) s += exp_fast(v[j] - ref);
+    for (int j = 0; j < kEach; ++j) s += exp2_fast(fmaf(v[j], kLog2e, shift));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
     if (lane == 0) {
@@ -286,35 +284,38 @@ __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, 
     if (threadIdx.x == 0) sm.count = 0;
     // Threads with two logits or more have two samples.
     const int sampled = wide ? n / kVec : max(0, n - kThreads);
-    uint32_t bound = block_bound<kThreads>(top[0], top[1], a.keep, min(sampled, kThreads) / 32, sm.bounds);
+    const uint32_t low = block_bound<kThreads>(inside(0) ? logit_bits(top[0]) : 0u, inside(1) ? logit_bits(top[1]) : 0u, a.keep, min(sampled, kThreads) / 32, sm.bounds);
+    const float bound = low > 1u ? float_from_order_key(low) : -INFINITY;
     if (threadIdx.x == 32) {
         float mm = -INFINITY, ss = 0.f;
         for (int w = 0; w < kThreads / 32; ++w) mm = fmaxf(mm, sm.m[w]);
         for (int w = 0; w < kThreads / 32; ++w) ss += sm.s[w] * expf(sm.m[w] == -INFINITY ? (mm == -INFINITY ? 0.f : -INFINITY) : sm.m[w] - mm);
         *stat = make_float2(mm, ss);
     }
-    auto push = [&](int j) {
+    auto push = [&](int j, uint32_t bits) {
         const int p = atomicAdd(&sm.count, 1);
-        if (p < kList) sm.list[p] = static_cast<uint64_t>(bits[j]) << 32 | static_cast<uint32_t>(~(c0 + at(j)));
+        if (p < kList) sm.list[p] = static_cast<uint64_t>(bits) << 32 | static_cast<uint32_t>(~(c0 + at(j)));
     };
 #pragma unroll
     for (int j = 0; j < kEach; ++j)
-        if (bits[j] >= bound) push(j);
+        if (!(v[j] < bound) && inside(j)) push(j, logit_bits(v[j]));
     __syncthreads();
     if (sm.count > kList) {
-        // Too many ties to list: the keep-th value, then how far its ties go.
-        bound = 0;
+        // Too many ties to list: the keep-th value, then how far its ties go. 0 where there is no logit (every logit's bits are above).
+        uint32_t bits[kEach], value = 0;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) bits[j] = inside(j) ? logit_bits(v[j]) : 0u;
 #pragma unroll 1
         for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t test = bound | 1u << bit;
+            const uint32_t test = value | 1u << bit;
             int above = 0;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) above += bits[j] >= test;
-            if (block_sum<kThreads>(above, sm.n) >= a.keep) bound = test;
+            if (block_sum<kThreads>(above, sm.n) >= a.keep) value = test;
         }
         int above = 0;
 #pragma unroll
-        for (int j = 0; j < kEach; ++j) above += bits[j] > bound;
+        for (int j = 0; j < kEach; ++j) above += bits[j] > value;
         const int ties = a.keep - block_sum<kThreads>(above, sm.n);  // wanted: 1 or more
         uint32_t last = 0;  // the largest place with fewer ties before it
 #pragma unroll 1
@@ -322,14 +323,14 @@ __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, 
             const uint32_t test = last | 1u << bit;
             above = 0;
 #pragma unroll
-            for (int j = 0; j < kEach; ++j) above += bits[j] == bound && at(j) < static_cast<int>(test);
+            for (int j = 0; j < kEach; ++j) above += bits[j] == value && at(j) < static_cast<int>(test);
             if (block_sum<kThreads>(above, sm.n) < ties) last = test;
         }
         if (threadIdx.x == 0) sm.count = 0;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
-            if (bits[j] > bound || (bits[j] == bound && static_cast<uint32_t>(at(j)) <= last)) push(j);
+            if (bits[j] > value || (bits[j] == value && static_cast<uint32_t>(at(j)) <= last)) push(j, bits[j]);
     }
     __syncthreads();
     const int count = min(sm.count, kList);

@@ -11,7 +11,7 @@
 //   searched bit by bit over value and token.
 // group stage: joins the rows' sums and ranks the lists' candidates in the same way. Up to 256 chunks the last block of a
 //   group to finish does it; with more, a block for each group in a second launch, in place when the chunks are done (4 rows x
-//   128256: 17.7 us a call with one launch, 21.7 with two, of which the GPU needs 11 and 9; 64 rows: 24.8 and 22.2).
+//   128256: 12.8 us a call with one launch, 14.8 with two; the GPU's part is 11 and 9).
 #include <cmath>
 
 #include "common/check.h"

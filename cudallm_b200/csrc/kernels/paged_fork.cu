@@ -6,7 +6,7 @@
 // references) does.
 //
 // One launch where plan and moves are small: every block makes the whole plan for itself, in shared memory, which costs no
-// more time than one block making it, and moves its share (the caller's thread needs 5 us instead of 8.5). Otherwise two: a plan kernel into
+// more time than one block making it, and moves its share (four beams: 14.1 us a call instead of 16.5). Otherwise two: a plan kernel into
 // the workspace and a move kernel over the GPU, in place when the plan is done.
 #include <algorithm>
 #include <atomic>

@@ -693,12 +693,11 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
 }
 
 // Joins the partials of items that were cut, in the order of their CTAs: block (c, h) those of head h of the item that ends in CTA
-// c's first segment. The block's warps take every eighth partial; the loads of each are independent of each other.
-constexpr int kJoinWarps = 8;
-template <typename X, int HD>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ Params p) {
+// c's first segment. The block's WARPS warps take the partials in turn; the loads of each are independent of each other.
+template <typename X, int HD, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) join_kernel(const __grid_constant__ Params p) {
     constexpr int V = HD / 32;  // dims of a lane
-    __shared__ float warp_m[kJoinWarps], warp_l[kJoinWarps], warp_o[kJoinWarps][HD];
+    __shared__ float warp_m[WARPS], warp_l[WARPS], warp_o[WARPS][HD];
     grid_dep_wait();
     const int4 head = __ldcg(reinterpret_cast<const int4*>(p.endings + blockIdx.x));
     const int parts = head.x, c0 = head.y, h = blockIdx.y;
@@ -710,11 +709,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
     for (int i = 0; i < V; ++i) o[i] = 0.f;
     auto part = [&](int c) { return p.parts + (static_cast<size_t>(c0 + c) * 2 + (c == 0)) * kSlotFloats; };
     constexpr int kAtOnce = 8;
-    for (int from = warp; from < parts; from += kAtOnce * kJoinWarps) {
+    for (int from = warp; from < parts; from += kAtOnce * WARPS) {
         float pm[kAtOnce], pl[kAtOnce], po[kAtOnce][V];
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
-            const int c = from + k * kJoinWarps;
+            const int c = from + k * WARPS;
             pm[k] = -INFINITY;
             if (c >= parts) continue;
             const float* src = part(c);
@@ -742,7 +741,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
         for (int i = 0; i < V; ++i) o[i] *= old;
 #pragma unroll
         for (int k = 0; k < kAtOnce; ++k) {
-            if (from + k * kJoinWarps >= parts) break;
+            if (from + k * WARPS >= parts) break;
             const float f = exp2_fast(pm[k] - ref);
             l = fmaf(f, pl[k], l);
 #pragma unroll
@@ -756,13 +755,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_cons
 #pragma unroll
     for (int i = 0; i < V; ++i) warp_o[warp][lane * V + i] = o[i];
     __syncthreads();
-    for (int d = threadIdx.x; d < p.head_dim; d += 32 * kJoinWarps) {
+    for (int d = threadIdx.x; d < p.head_dim; d += 32 * WARPS) {
         float mm = -INFINITY, ll = 0.f, v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) mm = fmaxf(mm, warp_m[w]);
+        for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, warp_m[w]);
         const float ref = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const float f = exp2_fast(warp_m[w] - ref);
             ll = fmaf(f, warp_l[w], ll);
             v = fmaf(f, warp_o[w][d], v);
@@ -821,7 +820,11 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
         launch_kernel(kernel, dim3(grid), dim3(kThreads), smem, stream, true, p);
         // Items of up to kUnit tiles are cut only where equal shares cut them, which takes more tiles than there are CTAs x kUnit.
         const bool can_cut = (cap + S::kTile - 1) / S::kTile > kUnit || static_cast<long long>(p.n_seq) * p.items > grid;
-        if (can_cut) launch_kernel(join_kernel<X, HD>, dim3(grid, std::min(p.group, S::kHeads)), dim3(32 * kJoinWarps), 0, stream, true, p);
+        if (!can_cut) continue;
+        // Up to 16 partials an item: blocks of 2 warps, of which an SM takes all that it gets at once (37 ragged sequences: 63.8 us with 8
+        // warps, 60.6 with 2); more: 8 warps (one of 32768 tokens, 55 partials: 19.5 us with 8, 20.6 with 2).
+        const bool few = grid <= 16LL * p.n_seq * p.items;
+        launch_kernel(few ? join_kernel<X, HD, 2> : join_kernel<X, HD, 8>, dim3(grid, std::min(p.group, S::kHeads)), dim3(few ? 64 : 256), 0, stream, true, p);
     }
 }
 

@@ -170,6 +170,14 @@ def test_attend_strided_and_broadcast_queries():
     assert torch.equal(a, cache.attend(packed[:, :8].contiguous(), _ints(table), _ints(lens)))
 
 
+def test_attend_more_rows_than_one_launch_takes():
+    rng = np.random.default_rng(7)
+    lens = [int(n) for n in rng.integers(0, 60, 2500)]
+    table, pages = _layout(lens, 16)
+    cache = _cache(1, pages, 1, 16, 64, F16)
+    _check_attend(cache, torch.randn((2500, 4, 64), device="cuda"), table, lens)
+
+
 def test_attend_peaked_and_tiny_scores():
     """One key far above the rest, at either end and inside; and scores of one size where the weights are all alike."""
     lens = [900] * 4
@@ -457,6 +465,42 @@ def test_compact(pages, share, order):
     np.testing.assert_array_equal(_np(cache.v), v0)
 
 
+@pytest.mark.parametrize("pages, layers, kv_heads", [(9000, 2, 2), (16384, 1, 1), (16385, 1, 1), (40000, 1, 1)])
+def test_compact_large_pools(pages, layers, kv_heads):
+    """Plans that do not fit one launch: many heads of pages to move, many pages."""
+    rng = np.random.default_rng(pages)
+    cache = _cache(layers, pages, kv_heads, 1, 8, F16)
+    refs = (rng.random(pages) < 0.6).astype(np.int32) * rng.integers(1, 3, pages).astype(np.int32)
+    tables = rng.integers(-1, pages, (3, 500)).astype(np.int32)
+    k0, v0 = _np(cache.k).copy(), _np(cache.v).copy()
+    t, r, live = cache.compact(_ints(tables), _ints(refs))
+    want_t, want_r, want_live, moves = R.compact_ref(tables, refs)
+    np.testing.assert_array_equal(_np(r), want_r)
+    np.testing.assert_array_equal(_np(t), want_t)
+    assert int(live) == want_live
+    src, dst = (np.array(x) for x in zip(*moves))
+    k0[:, dst], v0[:, dst] = k0[:, src], v0[:, src]
+    np.testing.assert_array_equal(_np(cache.k), k0)
+    np.testing.assert_array_equal(_np(cache.v), v0)
+
+
+@pytest.mark.parametrize("pages, rows, n_out, layers, width", [(20000, 40, 60, 1, 12), (3000, 40, 60, 40, 12), (3000, 600, 700, 1, 12), (3000, 20, 20, 1, 1500)])
+def test_fork_plans_that_do_not_fit_one_launch(pages, rows, n_out, layers, width):
+    rng = np.random.default_rng(rows)
+    page = 4
+    lens = rng.integers(0, 30, rows)
+    counts = [-(-int(n) // page) for n in lens]
+    table, at = np.full((rows, width), -1, np.int32), 0
+    ids = rng.permutation(pages)
+    for r, n in enumerate(counts):
+        table[r, :n] = ids[at:at + n]
+        at += n
+    refs = np.bincount(table[table >= 0], minlength=pages).astype(np.int32)
+    cache = _cache(layers, pages, 4, page, 8, F16)
+    for room in (1, 9):
+        _check_fork(cache, table, lens, refs, rng.integers(-1, rows, n_out), room)
+
+
 def test_compact_keeps_attention():
     lens = [100, 37, 200]
     table, pages = _layout(lens, 16, spare=40)
@@ -574,6 +618,47 @@ def test_beam_same_bits_in_a_graph_and_on_two_streams():
     torch.cuda.synchronize()
     for got in there + here + [out]:
         assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_a_step_in_a_graph():
+    """A whole step of beams (fork, append, attend, select) captured once and replayed on new inputs equals the same calls."""
+    G, W, heads, vocab = 2, 3, 8, 5000
+    rows = G * W
+    cache, other = (_cache(2, 200, 2, 8, 64, F16, fill=0.0) for _ in range(2))
+    rope = paged.Rope.make(64)
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *shape: torch.randn(shape, generator=gen, device="cuda")  # noqa: E731
+    state = cache.fork(*cache.rows(rows, 20), _ints(range(rows)), room=11)
+    state = (state[0], torch.full_like(state[1], 10), state[2])
+    qkv, logits, scores, parents = rand(rows, heads + 4, 64), rand(rows, vocab), rand(G, W), _ints([0, 0, 1, 3, 5, 5])
+
+    def step(c):
+        t, n, r, missing = c.fork(*state, parents, room=1)
+        outs = []
+        for layer in range(2):
+            q = c.append(qkv[:, :heads], qkv[:, heads:heads + 2], qkv[:, heads + 2:], n, t, rope, layer=layer)
+            outs += [q, c.attend(q, t, n + 1, layer=layer)]
+        return [t, n, r, missing, *outs, *paged.beam_select(logits, scores, keep=W), c.k, c.v]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(cache)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(cache)
+    for _ in range(3):
+        for x in (qkv, logits, scores):
+            x.copy_(torch.randn(x.shape, generator=gen, device="cuda"))
+        parents.copy_(_ints([0, 2, 2, 4, 3, 3]))
+        for c in (cache, other):
+            c.k.zero_()
+            c.v.zero_()
+        graph.replay()
+        want = step(other)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
 
 
 # ---- refusals ---------------------------------------------------------------------------------

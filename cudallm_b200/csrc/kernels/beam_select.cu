@@ -37,9 +37,23 @@ constexpr unsigned kAll = 0xffffffffu;
 // Rank bits of a logit: not a number counts as -inf, -0 as 0.
 __device__ __forceinline__ uint32_t logit_bits(float x) { return float_order_key(isnan(x) ? -INFINITY : x + 0.f); }
 
-// The first 16 bits of the r-th largest of the values a, b of a warp's lanes (0 = none, or fewer than r of them): a lower bound of it.
+// The r-th largest of the values a, b of a warp's lanes (0 = none, or fewer than r of them), or a lower bound of it: its first 16 bits where r
+// is above 8.
 __device__ __forceinline__ uint32_t warp_bound(uint32_t a, uint32_t b, int r) {
     uint32_t bound = 0;
+    if (r <= 8) {  // one largest after the other
+#pragma unroll 1
+        for (int i = 0; i < r; ++i) {
+            const uint32_t mine = max(a, b);
+            bound = __reduce_max_sync(kAll, mine);
+            const int owner = __ffs(__ballot_sync(kAll, mine == bound)) - 1;
+            if (static_cast<int>(threadIdx.x & 31) == owner) {
+                if (a == bound) a = 0;
+                else b = 0;
+            }
+        }
+        return bound;
+    }
 #pragma unroll
     for (int bit = 31; bit >= 16; --bit) {
         const uint32_t test = bound | 1u << bit;
@@ -286,11 +300,16 @@ __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, 
     const int sampled = wide ? n / kVec : max(0, n - kThreads);
     const uint32_t low = block_bound<kThreads>(inside(0) ? logit_bits(top[0]) : 0u, inside(1) ? logit_bits(top[1]) : 0u, a.keep, min(sampled, kThreads) / 32, sm.bounds);
     const float bound = low > 1u ? float_from_order_key(low) : -INFINITY;
-    if (threadIdx.x == 32) {
-        float mm = -INFINITY, ss = 0.f;
-        for (int w = 0; w < kThreads / 32; ++w) mm = fmaxf(mm, sm.m[w]);
-        for (int w = 0; w < kThreads / 32; ++w) ss += sm.s[w] * expf(sm.m[w] == -INFINITY ? (mm == -INFINITY ? 0.f : -INFINITY) : sm.m[w] - mm);
-        *stat = make_float2(mm, ss);
+    if (warp == 1) {  // the warps' sums as one
+        static_assert(kThreads / 32 == 8, "lanes 0 .. 7 have a warp's each");
+        const float wm = sm.m[lane & 7];
+        float mm = wm;
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(kAll, mm, o));
+        float ss = sm.s[lane & 7] * expf(wm == -INFINITY ? (mm == -INFINITY ? 0.f : -INFINITY) : wm - mm);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) ss += __shfl_xor_sync(kAll, ss, o);
+        if (lane == 0) *stat = make_float2(mm, ss);
     }
     auto push = [&](int j, uint32_t bits) {
         const int p = atomicAdd(&sm.count, 1);
@@ -345,7 +364,7 @@ __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, 
 
 // Block = chunk of a row. With `counts` (one zero for each group), the last block of a group to finish selects its best.
 template <typename X>
-__global__ void __launch_bounds__(kThreads, 5) beam_chunk_kernel(const __grid_constant__ cudallm_beam_args a, uint64_t* lists, float2* stats, int chunks, bool wide,
+__global__ void __launch_bounds__(kThreads, 6) beam_chunk_kernel(const __grid_constant__ cudallm_beam_args a, uint64_t* lists, float2* stats, int chunks, bool wide,
                                                                  unsigned* counts) {
     __shared__ union {
         ChunkRoom chunk;

@@ -9,9 +9,9 @@
 //   many rows). It leaves their maximum, their sum of exponentials and the sorted keys of their `keep` best. The maxima of 512
 //   pieces give a lower bound of the keep-th best; the few logits above it are ranked by counting. Where more than 256 are above it (ties, a masked vocabulary) the keep-th key itself is
 //   searched bit by bit over value and token.
-// group stage: joins the rows' sums and ranks the lists' candidates in the same way. Up to 256 chunks the last block of a
-//   group to finish does it; with more, a block for each group in a second launch, in place when the chunks are done (4 rows x
-//   128256: 12.8 us a call with one launch, 14.8 with two; the GPU's part is 11 and 9).
+// group stage: joins the rows' sums and ranks the lists' candidates in the same way. Up to 512 chunks the last block of a
+//   group to finish does it; with more, a block for each group in a second launch, in place when the chunks are done (us a call with one
+//   launch and with two: 4 rows x 128256 12.8 and 15.4, 32 rows 13.0 and 15.3, 64 rows 17.4 and 15.3).
 //
 // Measured (B200, graph replay): 64 rows x 128256, fp32, 23.1 us (1.4 TB/s; the instructions of a list, about 40 a logit and warp, bound it), bf16
 // with 40 rows finished 15.2 us; 4 rows 11.6 us.
@@ -34,7 +34,7 @@ constexpr int kChunk = kThreads * kEach;
 constexpr int kList = 256;  // candidates above the bound that are ranked by counting
 constexpr int kGroupThreads = 512;
 constexpr int kGroupList = 512;
-constexpr int kOneLaunch = 256;  // chunks of a call with a single launch
+constexpr int kOneLaunch = 512;  // chunks of a call with a single launch
 constexpr unsigned kAll = 0xffffffffu;
 
 // Rank bits of a logit: not a number counts as -inf, -0 as 0.

@@ -41,6 +41,7 @@ except ImportError:
 _X = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _KV = {torch.float16: 0, torch.bfloat16: 1}
 _INVALID_ARG = 1
+_INT_MAX = 2 ** 31 - 1
 _BEAM_COUNTERS = 16384  # CUDALLM_BEAM_COUNTER_BYTES
 
 
@@ -186,6 +187,7 @@ class PagedCache:
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         _need(k.dim() == 5 and k.shape == v.shape and k.dtype == v.dtype and k.dtype in _KV and k.is_cuda and k.device == v.device,
               "k and v must be fp16 or bf16 tensors [layers][pages][kv heads][page size][head dim] of one shape on one GPU")
+        _need(max(k.shape) <= _INT_MAX, "sizes must be below 2^31")
         _need(k.stride() == v.stride() and k.stride(4) == 1, "k and v must have the same strides, and a head's dims side by side")
         self.k, self.v, self.device = k, v, k.device
         self._index = k.device.index
@@ -251,6 +253,8 @@ class PagedCache:
         rows, width, stride = _table(tables, self.device, "tables")
         if rows != n:
             _refuse(f"tables has {rows} rows for {n} queries")
+        if not (0 <= layer < self.n_layers and 0 <= window <= _INT_MAX):
+            _refuse(f"layer must be in [0, {self.n_layers}), window not negative and below 2^31")
         a = self._attend
         a.lens = _int32(lens, self.device, (n,), "lens")
         if out is None:
@@ -278,6 +282,8 @@ class PagedCache:
         x = _X.get(k.dtype)
         if x is None:
             _refuse("q, k and v must be fp32, fp16 or bf16")
+        if not 0 <= layer < self.n_layers:
+            _refuse(f"layer must be in [0, {self.n_layers})")
         n, kv_heads, a.k_token_stride, a.k_head_stride = _heads(k, dev, k.dtype, dim, "k")
         nv, v_heads, a.v_token_stride, a.v_head_stride = _heads(v, dev, k.dtype, dim, "v")
         if kv_heads != self.n_kv_heads or v_heads != kv_heads or nv != n:
@@ -320,8 +326,8 @@ class PagedCache:
         `out` = such a tuple to write, which must not overlap the inputs (a program keeps two and swaps them)."""
         dev, a = self.device, self._fork
         n_rows, width, a.table_stride = _table(tables, dev, "tables")
-        if parents.dim() != 1:
-            _refuse("parents must be a vector")
+        if parents.dim() != 1 or not 0 <= room <= _INT_MAX:
+            _refuse("parents must be a vector, room not negative and below 2^31")
         n_out = parents.shape[0]
         a.lens = _int32(lens, dev, (n_rows,), "lens")
         a.refs = _int32(refs, dev, (self.n_pages,), "refs")
@@ -386,6 +392,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     row_stride, inner = logits.stride()
     if rows != groups * beams or (rows and vocab > 1 and inner != 1):
         _refuse("logits must have groups * beams rows with their values side by side")
+    if not (1 <= keep <= _INT_MAX and 0 <= eos <= _INT_MAX):
+        _refuse("keep must be positive, eos a token")
     a, ref = _beam_args()
     a.finished = None if finished is None else _int32(finished, dev, (groups, beams), "finished")
     if out is None:

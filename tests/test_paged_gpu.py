@@ -663,6 +663,20 @@ def test_a_step_in_a_graph():
 
 # ---- refusals ---------------------------------------------------------------------------------
 
+def test_numbers_beyond_32_bits_are_refused():
+    """They must not come out as other, valid numbers in the C structs."""
+    cache = _cache(2, 8, 2, 16, 64, F16)
+    t, n, r = cache.rows(2, 3)
+    q, k, pos = torch.zeros((2, 8, 64), device="cuda"), torch.zeros((2, 2, 64), device="cuda"), _ints([0, 0])
+    big = 2 ** 32
+    for call in (lambda: cache.attend(q, t, n, layer=big), lambda: cache.attend(q, t, n, window=big), lambda: cache.append(q, k, k, pos, t, None, layer=big + 1),
+                 lambda: cache.fork(t, n, r, pos, room=big), lambda: paged.beam_select(q[0], _f32([[0.0] * 8]), keep=big + 1),
+                 lambda: paged.beam_select(q[0], _f32([[0.0] * 8]), keep=1, finished=_ints([[0] * 8]), eos=big), lambda: cache.attend(q, t, n, scale=1e300)):
+        with pytest.raises(CudaLLMError) as e:
+            call()
+        assert e.value.code == 1
+
+
 def test_refusals():
     cache = _cache(2, 8, 2, 16, 64, F16)
     t, n, r = cache.rows(2, 3)

@@ -28,12 +28,16 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kEach = 16;  // pages of a thread in one pass over the references
-constexpr int kPass = kPlanThreads * kEach;
 constexpr int kMoveThreads = 256;
+// Plans of up to 16384 pages (and 1024 rows) are made by 256 threads, whose barriers cost less (four beams: 5.0 us on the GPU instead of 8.1).
+constexpr int kOneThreads = 256;
+constexpr int kOnePages = 16384;
+constexpr int kOneBlocks = 3;  // of the kernels that plan and move, on an SM
 constexpr int kSharedRows = 4096;  // rows whose counters fit the plan's shared memory
 constexpr unsigned kAll = 0xffffffffu;
 
-// Exclusive prefix sum of one value per thread over the block; `total` gets the sum. Barriers on both sides.
+// Exclusive prefix sum of one value per thread over a block; `total` gets the sum. Barriers on both sides.
+template <int THREADS>
 __device__ int block_scan(int v, int* sm, int& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int s = v;
@@ -45,13 +49,13 @@ __device__ int block_scan(int v, int* sm, int& total) {
     __syncthreads();
     if (lane == 31) sm[warp] = s;
     __syncthreads();
-    int w = sm[lane];  // every warp sums the warps' totals for itself
+    int w = lane < THREADS / 32 ? sm[lane] : 0;  // every warp sums the warps' totals for itself
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
+    for (int o = 1; o < THREADS / 32; o <<= 1) {
         const int t = __shfl_up_sync(kAll, w, o);
         if (lane >= o) w += t;
     }
-    total = __shfl_sync(kAll, w, 31);
+    total = __shfl_sync(kAll, w, THREADS / 32 - 1);
     const int before = __shfl_sync(kAll, w, (warp + 31) & 31);
     return s - v + (warp > 0 ? before : 0);
 }
@@ -144,26 +148,27 @@ __device__ __forceinline__ int row_len(const cudallm_pages& pg, const cudallm_fo
 }
 
 // The plan of a fork, by all threads of a block. `counters`: room for two ints for each of n_rows. Ends with a barrier.
+template <int THREADS>
 __device__ __forceinline__ void plan_fork(const cudallm_pages& pg, const cudallm_fork_args& a, const ForkPlan& s, int* counters, bool wide) {
     __shared__ int sm[32];
     __shared__ unsigned long long over;
     int refs[kEach];  // of the first pass, under way while the rows are looked at
     load_refs(a.refs, threadIdx.x * kEach, pg.n_pages, 1, wide, refs);
     int *children = counters, *first = counters + a.n_rows;
-    for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {
+    for (int r = threadIdx.x; r < a.n_rows; r += THREADS) {
         children[r] = 0;
         first[r] = INT_MAX;
     }
     if (threadIdx.x == 0) over = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < a.n_out; i += kPlanThreads) {
+    for (int i = threadIdx.x; i < a.n_out; i += THREADS) {
         const int p = a.parents[i];
         if (p >= 0 && p < a.n_rows) {
             atomicAdd(&children[p], 1);
             atomicMin(&first[p], i);
         }
     }
-    for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {
+    for (int r = threadIdx.x; r < a.n_rows; r += THREADS) {
         const int full = row_len(pg, a, r) / pg.page_size;
         const int* row = a.tables + r * a.table_stride;
         int held = full, open = -1;
@@ -175,13 +180,13 @@ __device__ __forceinline__ void plan_fork(const cudallm_pages& pg, const cudallm
         s.old[r] = {full, held, 0, open >= 0 && a.refs[open] == 1, open};
     }
     __syncthreads();
-    for (int r = threadIdx.x; r < a.n_rows; r += kPlanThreads) {  // a thread's own rows
+    for (int r = threadIdx.x; r < a.n_rows; r += THREADS) {  // a thread's own rows
         s.old[r].children = children[r];
         if (children[r] == 0) s.old[r].kept = 0;
     }
     __syncthreads();
     int base = 0;
-    for (int i0 = 0; i0 < a.n_out; i0 += kPlanThreads) {
+    for (int i0 = 0; i0 < a.n_out; i0 += THREADS) {
         const int i = i0 + threadIdx.x;
         int fresh = 0;
         OutRow o{-1, 0, 0, 0};
@@ -198,7 +203,7 @@ __device__ __forceinline__ void plan_fork(const cudallm_pages& pg, const cudallm
             }
         }
         int total;
-        o.start = base + block_scan(fresh, sm, total);
+        o.start = base + block_scan<THREADS>(fresh, sm, total);
         if (i < a.n_out) {
             s.out[i] = o;
             s.fresh[i] = fresh;
@@ -206,13 +211,13 @@ __device__ __forceinline__ void plan_fork(const cudallm_pages& pg, const cudallm
         base += total;
     }
     int found = 0;
-    for (int p0 = 0; p0 < pg.n_pages && found < base; p0 += kPass) {
+    for (int p0 = 0; p0 < pg.n_pages && found < base; p0 += (THREADS * kEach)) {
         const int p = p0 + threadIdx.x * kEach;
         if (p0 > 0) load_refs(a.refs, p, pg.n_pages, 1, wide, refs);
         int n = 0, total;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) n += refs[i] == 0;
-        int at = found + block_scan(n, sm, total);
+        int at = found + block_scan<THREADS>(n, sm, total);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             if (refs[i] == 0 && at < base) s.found[at] = p + i;
@@ -223,7 +228,7 @@ __device__ __forceinline__ void plan_fork(const cudallm_pages& pg, const cudallm
     found = min(found, base);
     __syncthreads();
     int copies = 0;
-    for (int i0 = 0; i0 < a.n_out; i0 += kPlanThreads) {
+    for (int i0 = 0; i0 < a.n_out; i0 += THREADS) {
         const int i = i0 + threadIdx.x;
         Copy c{0, 0, 0, 0};
         if (i < a.n_out) {
@@ -236,7 +241,7 @@ __device__ __forceinline__ void plan_fork(const cudallm_pages& pg, const cudallm
             }
         }
         int total;
-        const int at = copies + block_scan(c.tokens > 0, sm, total);
+        const int at = copies + block_scan<THREADS>(c.tokens > 0, sm, total);
         if (c.tokens > 0) s.copies[at] = c;
         copies += total;
     }
@@ -291,16 +296,17 @@ __device__ __forceinline__ void fork_copies(const cudallm_pages& pg, const ForkP
 }
 
 // Block 0 plans; the others copy the references, which the move kernel then changes.
-__global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
-                                                                 bool wide) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) fork_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, ForkPlan s,
+                                                            bool wide) {
     extern __shared__ int shared_counters[];
     grid_dep_wait();
     grid_dep_launch();
     if (blockIdx.x > 0) {
-        for (int p = (blockIdx.x - 1) * kPlanThreads + threadIdx.x; p < pg.n_pages; p += (gridDim.x - 1) * kPlanThreads) a.refs_out[p] = a.refs[p];
+        for (int p = (blockIdx.x - 1) * THREADS + threadIdx.x; p < pg.n_pages; p += (gridDim.x - 1) * THREADS) a.refs_out[p] = a.refs[p];
         return;
     }
-    plan_fork(pg, a, s, a.n_rows <= kSharedRows ? shared_counters : s.counters, wide);
+    plan_fork<THREADS>(pg, a, s, a.n_rows <= kSharedRows ? shared_counters : s.counters, wide);
     if (threadIdx.x == 0) *a.missing = s.totals[2];
 }
 
@@ -317,22 +323,22 @@ __global__ void __launch_bounds__(kMoveThreads) fork_move_kernel(const __grid_co
 }
 
 // The whole fork: block 0 writes the rows, the other blocks copy.
-__global__ void __launch_bounds__(kPlanThreads) fork_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, int rows, FastDiv by_row,
-                                                            bool wide) {
+__global__ void __launch_bounds__(kOneThreads) fork_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_fork_args a, int rows, FastDiv by_row,
+                                                           bool wide) {
     extern __shared__ __align__(16) char room[];
     const ForkPlan s = fork_plan(room, rows, kOneFound);
     grid_dep_wait();
     grid_dep_launch();
     if (blockIdx.x == 0) {
-        for (int p = threadIdx.x; p < pg.n_pages; p += kPlanThreads) a.refs_out[p] = a.refs[p];
+        for (int p = threadIdx.x; p < pg.n_pages; p += kOneThreads) a.refs_out[p] = a.refs[p];
     }
-    plan_fork(pg, a, s, s.counters, wide);
+    plan_fork<kOneThreads>(pg, a, s, s.counters, wide);
     if (blockIdx.x == 0) {
         if (threadIdx.x == 0) *a.missing = s.totals[2];
-        fork_rows(pg, a, s, rows, threadIdx.x, kPlanThreads);
+        fork_rows(pg, a, s, rows, threadIdx.x, kOneThreads);
     } else {
-        constexpr int kWarps = kPlanThreads / 32;
-        fork_copies<2>(pg, s, by_row, static_cast<long long>(blockIdx.x - 1) * kWarps + threadIdx.x / 32, static_cast<long long>(gridDim.x - 1) * kWarps);
+        constexpr int kWarps = kOneThreads / 32;
+        fork_copies<4>(pg, s, by_row, static_cast<long long>(blockIdx.x - 1) * kWarps + threadIdx.x / 32, static_cast<long long>(gridDim.x - 1) * kWarps);
     }
 }
 
@@ -347,29 +353,29 @@ __host__ __device__ inline CompactPlan compact_plan(void* memory, int n_pages) {
     int* p = static_cast<int*>(memory);
     return {p, p + 4, p + 4 + n_pages, p + 4 + n_pages + n_pages / 2};
 }
-constexpr int kOnePages = kPass;  // pages of a plan in shared memory
 
 // The plan of a compaction, by all threads of a block. Ends with a barrier.
+template <int THREADS>
 __device__ __forceinline__ void plan_compact(const cudallm_pages& pg, const cudallm_compact_args& a, const CompactPlan& s, bool wide) {
     __shared__ int sm[32];
     int refs[kEach], live = 0;
-    for (int p0 = 0; p0 < pg.n_pages; p0 += kPass) {
+    for (int p0 = 0; p0 < pg.n_pages; p0 += (THREADS * kEach)) {
         load_refs(a.refs, p0 + threadIdx.x * kEach, pg.n_pages, 0, wide, refs);
         int n = 0, total;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) n += refs[i] > 0;
-        block_scan(n, sm, total);
+        block_scan<THREADS>(n, sm, total);
         live += total;
     }
     int holes = 0, movers = 0;
-    for (int p0 = 0; p0 < pg.n_pages; p0 += kPass) {
+    for (int p0 = 0; p0 < pg.n_pages; p0 += (THREADS * kEach)) {
         const int p = p0 + threadIdx.x * kEach;
-        if (pg.n_pages > kPass) load_refs(a.refs, p, pg.n_pages, 0, wide, refs);
+        if (pg.n_pages > (THREADS * kEach)) load_refs(a.refs, p, pg.n_pages, 0, wide, refs);
         int n = 0, total;  // holes in the low half, movers in the high one: a pass has at most 16384 of each
-        static_assert(kPass < 1 << 15, "two counts in one int");
+        static_assert(THREADS * kEach < 1 << 15, "two counts in one int");
 #pragma unroll
         for (int i = 0; i < kEach; ++i) n += refs[i] > 0 ? (p + i >= live) << 16 : p + i < live;
-        const int at = block_scan(n, sm, total);
+        const int at = block_scan<THREADS>(n, sm, total);
         int h = holes + (at & 0xffff), m = movers + (at >> 16);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
@@ -380,7 +386,7 @@ __device__ __forceinline__ void plan_compact(const cudallm_pages& pg, const cuda
         movers += total >> 16;
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < movers; k += kPlanThreads) s.to[s.src[k]] = s.dst[k];
+    for (int k = threadIdx.x; k < movers; k += THREADS) s.to[s.src[k]] = s.dst[k];
     if (threadIdx.x == 0) {
         s.totals[0] = live;
         s.totals[1] = movers;
@@ -412,11 +418,12 @@ __device__ __forceinline__ void move_compact(const cudallm_pages& pg, const cuda
     }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
-                                                                    bool wide) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) compact_plan_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
+                                                               bool wide) {
     grid_dep_wait();
     grid_dep_launch();
-    plan_compact(pg, a, s, wide);
+    plan_compact<THREADS>(pg, a, s, wide);
 }
 
 __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, CompactPlan s,
@@ -425,14 +432,14 @@ __global__ void __launch_bounds__(kMoveThreads) compact_move_kernel(const __grid
     move_compact<4>(pg, a, s, by_row, static_cast<long long>(blockIdx.x) * kMoveThreads + threadIdx.x, static_cast<long long>(gridDim.x) * kMoveThreads);
 }
 
-__global__ void __launch_bounds__(kPlanThreads) compact_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, FastDiv by_row,
-                                                               bool wide) {
+__global__ void __launch_bounds__(kOneThreads) compact_kernel(const __grid_constant__ cudallm_pages pg, const __grid_constant__ cudallm_compact_args a, FastDiv by_row,
+                                                              bool wide) {
     extern __shared__ __align__(16) char room[];
     const CompactPlan s = compact_plan(room, pg.n_pages);
     grid_dep_wait();
     grid_dep_launch();
-    plan_compact(pg, a, s, wide);
-    move_compact<2>(pg, a, s, by_row, static_cast<long long>(blockIdx.x) * kPlanThreads + threadIdx.x, static_cast<long long>(gridDim.x) * kPlanThreads);
+    plan_compact<kOneThreads>(pg, a, s, wide);
+    move_compact<4>(pg, a, s, by_row, static_cast<long long>(blockIdx.x) * kOneThreads + threadIdx.x, static_cast<long long>(gridDim.x) * kOneThreads);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -450,17 +457,18 @@ void launch_paged_fork(const cudallm_pages& pg, const cudallm_fork_args& a, cuda
     const bool wide = aligned16(a.refs);
     const long long heads = static_cast<long long>(a.n_out) * pg.n_layers * pg.n_kv_heads;  // most that are copied
     const long long most_new = a.n_out * (2LL + a.room / pg.page_size);
-    if (pg.n_pages <= kPass && rows <= kOneRows && most_new <= kOneFound && static_cast<long long>(rows) * a.table_width <= kOneEntries &&
+    if (pg.n_pages <= kOnePages && rows <= kOneRows && most_new <= kOneFound && static_cast<long long>(rows) * a.table_width <= kOneEntries &&
         heads <= kOneHeads) {
-        constexpr int kWarps = kPlanThreads / 32;
-        const int blocks = 1 + static_cast<int>(std::min<long long>(sms - 1, std::max<long long>(1, (heads + kWarps - 1) / kWarps)));
-        launch_kernel(fork_kernel, dim3(blocks), dim3(kPlanThreads), fork_plan_bytes(rows, kOneFound), stream, true, pg, a, rows, by_row, wide);
+        constexpr int kWarps = kOneThreads / 32;
+        const int blocks = 1 + static_cast<int>(std::min<long long>(kOneBlocks * sms - 1, std::max<long long>(1, (heads + kWarps - 1) / kWarps)));
+        launch_kernel(fork_kernel, dim3(blocks), dim3(kOneThreads), fork_plan_bytes(rows, kOneFound), stream, true, pg, a, rows, by_row, wide);
         return;
     }
     const ForkPlan s = fork_plan(a.workspace, rows, pg.n_pages);
-    const int copiers = std::min(sms, (pg.n_pages + kPlanThreads - 1) / kPlanThreads);  // of the references
+    const bool small = pg.n_pages <= kOnePages && rows <= kPlanThreads;
+    const int threads = small ? kOneThreads : kPlanThreads, copiers = std::min(sms, (pg.n_pages + threads - 1) / threads);  // of the references
     const size_t smem = a.n_rows <= kSharedRows ? 8 * static_cast<size_t>(a.n_rows) : 0;
-    launch_kernel(fork_plan_kernel, dim3(1 + copiers), dim3(kPlanThreads), smem, stream, true, pg, a, s, wide);
+    launch_kernel(small ? fork_plan_kernel<kOneThreads> : fork_plan_kernel<kPlanThreads>, dim3(1 + copiers), dim3(threads), smem, stream, true, pg, a, s, wide);
     if (rows == 0) return;
     const int movers = static_cast<int>(std::min<long long>(8LL * sms, (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
     const long long entries = static_cast<long long>(rows) * a.table_width;
@@ -476,12 +484,14 @@ void launch_paged_compact(const cudallm_pages& pg, const cudallm_compact_args& a
         const size_t smem = compact_plan_bytes(pg.n_pages);
         static std::atomic<uint64_t> allowed{0};  // devices on which the kernel may use its shared memory
         allow_shared(compact_kernel, static_cast<int>(compact_plan_bytes(kOnePages)), allowed);
-        const long long most = 1 + (heads + kPlanThreads / 32 - 1) / (kPlanThreads / 32);
-        launch_kernel(compact_kernel, dim3(static_cast<int>(std::min<long long>(num_sms(), most))), dim3(kPlanThreads), smem, stream, true, pg, a, by_row, wide);
+        const long long most = 1 + (heads + kOneThreads / 32 - 1) / (kOneThreads / 32);
+        launch_kernel(compact_kernel, dim3(static_cast<int>(std::min<long long>(kOneBlocks * num_sms(), most))), dim3(kOneThreads), smem, stream, true, pg, a, by_row, wide);
         return;
     }
     const CompactPlan s = compact_plan(a.workspace, pg.n_pages);
-    launch_kernel(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, true, pg, a, s, wide);
+    const bool small = pg.n_pages <= kOnePages;
+    launch_kernel(small ? compact_plan_kernel<kOneThreads> : compact_plan_kernel<kPlanThreads>, dim3(1), dim3(small ? kOneThreads : kPlanThreads), 0, stream, true,
+                  pg, a, s, wide);
     const int blocks = static_cast<int>(std::min<long long>(8LL * num_sms(), 1 + (heads + kMoveThreads / 32 - 1) / (kMoveThreads / 32)));
     launch_kernel(compact_move_kernel, dim3(blocks), dim3(kMoveThreads), 0, stream, true, pg, a, s, by_row);
 }

@@ -163,15 +163,16 @@ struct Unit {
     }
 };
 
-// Units of 8 pairs or of fp32 are loaded one at a time, by 4 blocks on an SM; smaller ones two at a time, by 5. Measured on 16383 tokens (us):
-// bf16, 48 heads of 128 dims, 64 of them rotated interleaved: 4 loads and 3 blocks 91, 2 and 5 81, 1 and 5 84; all rotated in halves: 2 and 3
-// 80, 2 and 4 110 (spills), 1 and 4 80; fp32, 64 dims in halves: 2 and 3 109, 1 and 4 70.
+// Units of 8 pairs or of fp32 are loaded one at a time, others two at a time, by 4 (8 pairs) or 5 blocks on an SM. Measured on 16383 tokens
+// of 48 heads (us; loads at a time and blocks): bf16 x 128, 64 rotated interleaved: 4 and 3 91, 2 and 5 81, 1 and 5 84; bf16 x 128 in halves:
+// 2 and 3 80, 2 and 4 110 (spills), 1 and 4 80, 1 and 5 86; fp32 x 64 in halves: 2 and 3 109, 1 and 4 70, 1 and 5 85; interleaved: 1 and 4 73,
+// 1 and 5 67.
 template <typename X, Layout L>
-constexpr bool few_registers = L == Layout::kHalves || (L == Layout::kInterleaved && sizeof(X) == 4);
+constexpr bool one_load = L == Layout::kHalves || (L == Layout::kInterleaved && sizeof(X) == 4);
 
 template <typename X, typename KV, Layout L>
-__global__ void __launch_bounds__(kThreads, few_registers<X, L> ? 4 : 5) append_kernel(const __grid_constant__ Params p) {
-    constexpr int kItems = few_registers<X, L> ? 1 : 2;  // heads of a thread whose loads are under way together
+__global__ void __launch_bounds__(kThreads, L == Layout::kHalves ? 4 : 5) append_kernel(const __grid_constant__ Params p) {
+    constexpr int kItems = one_load<X, L> ? 1 : 2;  // heads of a thread whose loads are under way together
     __shared__ __align__(16) float cos[kTokens][128], sin[kTokens][128];
     __shared__ long long slots[kTokens];  // where the token's keys go; -1: nowhere, -2: padding
     const cudallm_append_args& a = p.a;

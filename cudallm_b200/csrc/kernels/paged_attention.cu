@@ -26,7 +26,7 @@
 // enough here, and its operands stay in registers between the two products; tcgen05 tiles of 64 or 128 rows would be padding for 8 heads.
 //
 // Measured (B200, graph replay): 32 heads on 8 key heads x 64, fp32 on bf16: 64 sequences of 512..767 tokens 25.6 us (3.3 TB/s), of 2048
-// 51.4 us (5.2 TB/s); one of 32768 19.5 us (3.4 TB/s); 32 on 4 x 128, 37 ragged sequences of up to 8111 60.6 us (5.1 TB/s). About 10 us of
+// 51.4 us (5.2 TB/s); one of 32768 19.5 us (3.4 TB/s); 32 on 4 x 128, 37 ragged sequences of up to 8111 60.4 us (5.1 TB/s). About 9 us of
 // each are the chain length - entry - page at the start, the last CTA and the join.
 #include <algorithm>
 #include <atomic>

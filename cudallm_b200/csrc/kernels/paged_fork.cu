@@ -6,11 +6,11 @@
 // references) does.
 //
 // One launch where plan and moves are small: every block makes the whole plan for itself, in shared memory, which costs no
-// more time than one block making it, and moves its share (four beams: 14.1 us a call instead of 16.5). Otherwise two: a plan kernel into
+// more time than one block making it, and moves its share (four beams: 13.7 us a call instead of 16). Otherwise two: a plan kernel into
 // the workspace and a move kernel over the GPU, in place when the plan is done.
 //
-// Measured (B200, graph replay): 128 rows, 64 tails of 16 layers (69 MB copied) 32.5 us, of which the move is 21.3 (6.5 TB/s); 750 pages
-// of 16 layers compacted (393 MB) 132 us (6.0 TB/s); four beams 8.1 us.
+// Measured (B200, graph replay): 128 rows, 64 tails of 16 layers (69 MB copied) 31.2 us, of which the move is 21.3 (6.5 TB/s); 750 pages
+// of 16 layers compacted (393 MB) 131 us (6.0 TB/s); four beams 5.1 us.
 #include <algorithm>
 #include <atomic>
 #include <climits>

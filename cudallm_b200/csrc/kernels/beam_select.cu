@@ -288,10 +288,9 @@ __device__ __forceinline__ void list_chunk(const cudallm_beam_args& a, int row, 
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(kAll, m, o));
     const float ref = m == -INFINITY ? 0.f : m;
     constexpr float kLog2e = 1.4426950408889634f;
-    const float shift = -ref * kLog2e;
-    float s = 0.f;
+    float s = 0.f;  // x - m first: scaled apart, the two would differ by the rounding of m, which passes any exponent where all is masked by a large number
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) s += exp2_fast(fmaf(v[j], kLog2e, shift));
+    for (int j = 0; j < kEach; ++j) s += exp2_fast((v[j] - ref) * kLog2e);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
     if (lane == 0) {

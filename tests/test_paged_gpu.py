@@ -587,6 +587,22 @@ def test_beam_masked_and_poisoned_rows():
     _check_beam(torch.full((2, 3000), -inf, device="cuda"), [[-inf, 0.0]], 4)
 
 
+@pytest.mark.parametrize("x, ban", [(F32, -1e4), (F32, -1e9), (F32, -1e10), (F32, -1e30), (F32, -3.4028234663852886e38), (BF16, -1e30), (BF16, -3.3895313892515355e38),
+                                    (F16, -65504.0)])
+def test_beam_tokens_masked_by_large_numbers(x, ban):
+    """Most tokens of a row masked by a number, so that whole parts of it hold nothing else: as if they were masked by -inf."""
+    vocab, keep = 30011, 9
+    logits = torch.randn((4, vocab), device="cuda").to(x)
+    banned = torch.ones(vocab, dtype=torch.bool, device="cuda")
+    banned[torch.arange(40, device="cuda") * 7 + 17000] = False
+    scores = _f32([[-1.0, -2.0], [-3.0, -3.0]])
+    got = paged.beam_select(logits.masked_fill(banned, ban), scores, keep=keep)
+    ref = paged.beam_select(logits.masked_fill(banned, -float("inf")), scores, keep=keep)
+    assert bool(torch.isfinite(got[0]).all()) and all(torch.equal(a, b) for a, b in zip(got, ref))
+    _check_beam(logits.masked_fill(banned, -float("inf")), _np(scores), keep)
+    _check_beam(torch.full((2, vocab), ban, dtype=x, device="cuda"), [[0.0, -1.0]], keep)  # every token
+
+
 def test_beam_finished_rows():
     x = torch.randn((8, 3000), device="cuda")
     x[3] = float("nan")  # a finished beam's row is not read

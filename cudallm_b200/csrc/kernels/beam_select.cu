@@ -13,8 +13,8 @@
 //   group to finish does it; with more, a block for each group in a second launch, in place when the chunks are done (us a call with one
 //   launch and with two: 4 rows x 128256 12.8 and 15.4, 32 rows 13.0 and 15.3, 64 rows 17.4 and 15.3).
 //
-// Measured (B200, graph replay): 64 rows x 128256, fp32, 23.1 us (1.4 TB/s; the instructions of a list, about 40 a logit and warp, bound it), bf16
-// with 40 rows finished 15.2 us; 4 rows 11.6 us.
+// Measured (B200, graph replay): 64 rows x 128256, fp32, 22.9 us (1.4 TB/s; the instructions of a list, about 40 a logit and warp, bound it), bf16
+// with 40 rows finished 15.6 us; 4 rows 12.2 us.
 #include <cmath>
 
 #include "common/check.h"

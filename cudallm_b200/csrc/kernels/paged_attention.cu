@@ -20,8 +20,8 @@
 // Arithmetic. m16n8k16 matrix instructions with fp32 accumulators, 8 query heads a group: the second 8 rows of the
 // 16-row operand are free, so they carry a second plane of it. Scores: q as one plane of the cache's type when it has
 // that type, else as its rounding and the rounding of the rest (fp16: 22 bits; bf16: a third plane makes 24 bits for
-// fp32 queries). Weights: p likewise in two planes (three for fp32 results over bf16), so that rounding p never shows
-// in the result. Each tile's product starts from zero and is added to the running fp32 output outside of the
+// fp32 queries). Weights: p likewise in two planes (fp16: 22 bits of weights brought up to 2^15; bf16: 16 bits, a third plane
+// makes 24 for fp32 results). Each tile's product starts from zero and is added to the running fp32 output outside of the
 // tensor core, whose additions truncate. The matrix work is below a fifth of the tensor pipe's time, so the legacy instruction is fast
 // enough here, and its operands stay in registers between the two products; tcgen05 tiles of 64 or 128 rows would be padding for 8 heads.
 //
@@ -73,6 +73,7 @@ struct Params {
     Ending* endings;  // [CTA]
     long long q_seq_stride, q_head_stride, table_stride, page_stride, head_stride, token_stride;  // elements
     float scale2;                                                                                  // scale * log2(e)
+    float lse_unit;                                                                                // 2^-kLift
     int n_seq, n_heads, n_pages, page_size, table_width, head_dim, window;
     int group;      // query heads per key head
     int per_head;   // items per key head (groups of 8 HG query heads)
@@ -168,6 +169,10 @@ struct Shape {
     static constexpr int kQPlanes = std::is_same_v<X, KV> ? 1 : kBf16 && kF32 ? 3 : 2;
     static constexpr int kPPlanes = kBf16 && kF32 ? 3 : 2;
     static constexpr bool kScaleQ = !kBf16 && kQPlanes > 1;
+    // Weights are exp2(x - max + kLift). fp16's grid ends at 2^-24: planes of weights up to 1 would lose all that is 17 nats below the maximum, and
+    // digits from 10 nats on; with the largest at 2^15 what is lost is 2^-40 of it (output error under one token 17 nats above 32767 others:
+    // 0.19 without, 5e-8 with the lift). Sums and outputs carry the factor until the one is divided by the other.
+    static constexpr float kLift = kBf16 ? 0.f : 15.f;
     static constexpr int kTile = HD == 64 ? 32 : 16;  // tokens
     static constexpr int kStages = HD == 256 || HG == 2 ? 3 : 2;
     static constexpr int kCtas = HD == 256 ? 1 : HG == 2 ? 2 : 3;  // resident on an SM, by shared memory and registers
@@ -569,7 +574,9 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        x[n][e] = exp2_fast(x[n][e] - ref);
+                        x[n][e] -= ref;  // exact near the maximum, which ref - kLift would not be
+                        if constexpr (S::kLift != 0.f) x[n][e] += S::kLift;
+                        x[n][e] = exp2_fast(x[n][e]);
                         sum += x[n][e];
                     }
                 }
@@ -680,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
                             part[row] = mm;
                             part[16 + row] = ll;
                         } else if (p.lse != nullptr) {
-                            p.lse[row0 + row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
+                            p.lse[row0 + row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll * p.lse_unit)) : -INFINITY;
                         }
                     }
                 }
@@ -772,7 +779,7 @@ __global__ void __launch_bounds__(32 * WARPS) join_kernel(const __grid_constant_
             v = fmaf(f, warp_o[w][d], v);
         }
         static_cast<X*>(p.out)[row * p.head_dim + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
-        if (d == 0 && p.lse != nullptr) p.lse[row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll)) : -INFINITY;
+        if (d == 0 && p.lse != nullptr) p.lse[row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll * p.lse_unit)) : -INFINITY;
     }
 }
 
@@ -792,6 +799,7 @@ void launch_shape(const cudallm_pages& pg, const cudallm_attend_args& a, cudaStr
     p.head_stride = pg.head_stride;
     p.token_stride = pg.token_stride;
     p.scale2 = a.scale * kLog2e;
+    p.lse_unit = std::exp2(-S::kLift);
     p.n_heads = a.n_heads;
     p.n_pages = pg.n_pages;
     p.page_size = pg.page_size;

@@ -206,6 +206,37 @@ def test_attend_query_magnitudes(size):
     _check_attend(cache, q, table, lens, scale=0.125 / size)
 
 
+def _tail_case(gap, rows, length, seed=0):
+    """Rows over the same pages: a first token `gap` nats above all others with a value of 0, the others' values of one sign."""
+    page, dim = 64, 64
+    table, pages = _layout([length], page)
+    cache = _cache(1, pages, 1, page, dim, F16, seed=seed)
+    q = torch.randn(dim, generator=torch.Generator(device="cuda").manual_seed(seed + 1), device="cuda")
+    cache.k.mul_(0.05)
+    cache.v.abs_().add_(0.5)
+    cache.k[0, int(table[0][0]), 0, 0] = q * (gap / (dim ** -0.5 * float(q @ q)))
+    cache.v[0, int(table[0][0]), 0, 0] = 0.0
+    return cache, q.expand(rows, 4, dim), np.repeat(table, rows, 0), [length] * rows
+
+
+@pytest.mark.parametrize("x", [F32, F16, BF16])
+@pytest.mark.parametrize("gap", [10, 12, 14, 16, 17, 18, 20])
+@pytest.mark.parametrize("rows, length", [(1, 32768), (600, 8192)])
+def test_attend_many_small_weights_over_fp16_pages(x, gap, rows, length):
+    """The tail of a softmax under one large weight, in cut rows and in whole ones: what is left of the output is that tail, and has to keep its
+    digits. A weight is off by 2 E (score, sum) and by the rounding of its two planes: 2^-22 of itself and, as the largest is 2^15 and fp16's
+    grid 2^-24, 2^-40 of the largest; the lse as everywhere."""
+    cache, q, table, lens = _tail_case(gap, rows, length)
+    q = q.to(x)
+    out, lse = cache.attend(q, _ints(table), _ints(lens), with_lse=True)
+    ref, ref_lse, size = R.attend64(_np(q[:1]), _np(cache.k[0]), _np(cache.v[0]), table[:1], lens[:1])
+    e = (8 * EPS * np.sqrt(cache.head_dim) * size)[..., None]
+    tol = (2 * e + 8 * EPS * np.sqrt(length) + 2.0 ** -22) * np.abs(ref) + length * 2.0 ** -40 * np.abs(_np(cache.v)).max()
+    many = lambda a: np.broadcast_to(a, (rows, *a.shape[1:]))  # noqa: E731
+    _within(out, many(ref), many(tol))
+    _within(lse, many(ref_lse), many(e[..., 0] + 8 * EPS * np.sqrt(length) + 2 * EPS * np.abs(ref_lse)))
+
+
 def test_attend_offsets_past_32_bits():
     """Pages more than 2^32 elements into the pool."""
     page, dim, pages = 64, 128, 2 ** 32 // (64 * 128) + 300

@@ -383,11 +383,12 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
             float shrink = 1.f;
             q_scale[hg] = p.scale2;
             if constexpr (S::kScaleQ) {
-                // fp16 planes: the head is brought to 1 <= max|q| < 2 by a power of two, which the scale gives back.
+                // fp16 planes: the head is brought to 2^14 <= max|q| < 2^15 by a power of two, which the scale gives back; what fp16's grid
+                // of 2^-24 takes from the smallest dims is then below 2^-39 of the largest one.
                 float top = 0.f;
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) top = fmaxf(top, q_tops[w * 8 * HG + hg * 8 + g]);
-                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 1), 253) - 127;
+                const int e = min(max(static_cast<int>(__float_as_uint(top) >> 23), 15), 254) - 127 - 14;  // -126 .. 113: both powers are normal
                 shrink = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
                 q_scale[hg] *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
             }

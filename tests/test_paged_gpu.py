@@ -237,6 +237,21 @@ def test_attend_many_small_weights_over_fp16_pages(x, gap, rows, length):
     _within(lse, many(ref_lse), many(e[..., 0] + 8 * EPS * np.sqrt(length) + 2 * EPS * np.abs(ref_lse)))
 
 
+@pytest.mark.parametrize("x", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("big, rest", [(64.0, 1.0), (4096.0, 1.0), (65536.0, 1.0), (3e38, 1e36), (1e-30, 1e-30)])
+def test_attend_queries_with_one_large_dim(x, dim, big, rest):
+    """One dim of the query far above the others where the keys are 0, so that the others alone make the scores: they are held to the same tolerance
+    as without it. And queries at both ends of fp32's range."""
+    lens = [700, 40]
+    table, pages = _layout(lens, 16)
+    cache = _cache(1, pages, 2, 16, dim, F16)
+    cache.k[..., 3] = 0.0
+    q = rest * torch.randn((2, 8, dim), generator=torch.Generator(device="cuda").manual_seed(5), device="cuda")
+    q[..., 3] = big
+    _check_attend(cache, q.to(x), table, lens, scale=dim ** -0.5 / rest)
+
+
 def test_attend_offsets_past_32_bits():
     """Pages more than 2^32 elements into the pool."""
     page, dim, pages = 64, 128, 2 ** 32 // (64 * 128) + 300

@@ -661,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
                         ll = fmaf(f[w], join_l[w * 8 + g], ll);
                     }
                     const int row = hg * 8 + g;
-                    const float norm = !whole_item ? 1.f : ll > 0.f ? 1.f / ll : 0.f;
+                    const float norm = !whole_item ? 1.f : ll == 0.f ? 0.f : 1.f / ll;  // scores that are not numbers make ll one, too
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         float v[4];
@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(kThreads, Shape<X, KV, HD, HG>::kCtas) attend_
                             part[row] = mm;
                             part[16 + row] = ll;
                         } else if (p.lse != nullptr) {
-                            p.lse[row0 + row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll * p.lse_unit)) : -INFINITY;
+                            p.lse[row0 + row] = ll == 0.f ? -INFINITY : fmaf(mm, kLn2, logf(ll * p.lse_unit));
                         }
                     }
                 }
@@ -779,8 +779,8 @@ __global__ void __launch_bounds__(32 * WARPS) join_kernel(const __grid_constant_
             ll = fmaf(f, warp_l[w], ll);
             v = fmaf(f, warp_o[w][d], v);
         }
-        static_cast<X*>(p.out)[row * p.head_dim + d] = from_float<X>(ll > 0.f ? v / ll : 0.f);
-        if (d == 0 && p.lse != nullptr) p.lse[row] = ll > 0.f ? fmaf(mm, kLn2, logf(ll * p.lse_unit)) : -INFINITY;
+        static_cast<X*>(p.out)[row * p.head_dim + d] = from_float<X>(ll == 0.f ? 0.f : v / ll);
+        if (d == 0 && p.lse != nullptr) p.lse[row] = ll == 0.f ? -INFINITY : fmaf(mm, kLn2, logf(ll * p.lse_unit));
     }
 }
 

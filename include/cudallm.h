@@ -276,7 +276,8 @@ typedef struct {
 /* Attention of one new token per sequence over its pages: out[b][h] = softmax_t(scale q.k_t) v over the cached
  * positions max(0, lens[b] - window) <= t < lens[b] (window 0: all; lens outside [0, table_width * page_size] are
  * clamped to it) whose page exists; n_heads / n_kv_heads query heads share a key head. lse (or NULL): the natural
- * logarithm of the sum of the exponentials. No position left: out 0, lse -inf. Scores, statistics and sums are fp32.
+ * logarithm of the sum of the exponentials. No position left: out 0, lse -inf; a score that is not a number: out and
+ * lse of its head are not numbers either. Scores, statistics and sums are fp32.
  * q [n_seq][n_heads][head_dim] has its own strides, out and lse are contiguous; out has q's type and must not
  * overlap q. Values in unused slots of a page do not matter; keys and values of used ones must be finite. */
 typedef struct {

@@ -252,6 +252,26 @@ def test_attend_queries_with_one_large_dim(x, dim, big, rest):
     _check_attend(cache, q.to(x), table, lens, scale=dim ** -0.5 / rest)
 
 
+@pytest.mark.parametrize("x, kv", [(F32, F16), (F32, BF16), (F16, F16), (BF16, BF16), (BF16, F16)])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 64), (8, 4, 128), (32, 2, 128), (6, 2, 256)])
+def test_attend_queries_that_are_not_numbers(x, kv, heads, kv_heads, dim):
+    """Their heads are not numbers either, out and lse alike, in rows that are cut and rows that are whole; every other head keeps its bits, and a row
+    without a token is 0 and -inf as ever."""
+    lens = [20000, 1, 700, 0, 64]
+    table, pages = _layout(lens, 16)
+    cache = _cache(1, pages, kv_heads, 16, dim, kv)
+    q = torch.randn((len(lens), heads, dim), generator=torch.Generator(device="cuda").manual_seed(2), device="cuda").to(x)
+    bad = torch.zeros((len(lens), heads), dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[1, 0] = bad[2, heads - 1] = bad[3, 2] = bad[4, 3] = bad[4, 4] = True
+    dirty = q.clone()
+    dirty[..., dim // 2] = torch.where(bad, float("nan"), q[..., dim // 2])
+    ref, ref_lse = cache.attend(q, _ints(table), _ints(lens), with_lse=True)
+    out, lse = cache.attend(dirty, _ints(table), _ints(lens), with_lse=True)
+    bad[3] = False
+    assert bool(torch.isnan(out[bad]).all()) and bool(torch.isnan(lse[bad]).all())
+    assert torch.equal(out[~bad], ref[~bad]) and torch.equal(lse[~bad], ref_lse[~bad])
+
+
 def test_attend_offsets_past_32_bits():
     """Pages more than 2^32 elements into the pool."""
     page, dim, pages = 64, 128, 2 ** 32 // (64 * 128) + 300

@@ -28,9 +28,15 @@ KV_DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
 PREFILL_ROWS = 512  # prompt tokens of one pass
 
 
+def pool_pages(rows: int, max_seq_len: int, page_size: int) -> int:
+    """Pages with which any search of `rows` sequences of up to `max_seq_len` tokens succeeds: all that the rows can hold, and one more a
+    row, since a step's new pages are found before those of the beams that end in it are free."""
+    return rows * (-(-max_seq_len // page_size) + 1)
+
+
 class BeamSearch:
     """Beam search with a model's weights and a pool of pages for up to `rows` sequences (prompts * beams) of up to
-    `max_seq_len` tokens (0: the file header's value)."""
+    `max_seq_len` tokens (0: the file header's value); n_pages 0: as many as any search of that size can need."""
 
     def __init__(self, path: Path | str, *, rows: int = 16, max_seq_len: int = 0, page_size: int = 16, n_pages: int = 0,
                  kv_dtype: str = "fp16", device: str = "cuda"):
@@ -65,8 +71,8 @@ class BeamSearch:
                        for p in (f"layers.{i}." for i in range(self.n_layers))]
         self.rope = Rope(vector("rope.inv_freq"))
         self.rows, self.width = rows, -(-self.max_seq_len // page_size)
-        self.cache = PagedCache.allocate(self.n_layers, n_pages or rows * self.width + 1, self.kv_heads, page_size, self.head_dim,
-                                         dtype=KV_DTYPES[kv_dtype], device=self.device)
+        self.cache = PagedCache.allocate(self.n_layers, n_pages or pool_pages(rows, self.max_seq_len, page_size), self.kv_heads, page_size,
+                                         self.head_dim, dtype=KV_DTYPES[kv_dtype], device=self.device)
 
     def _norm(self, x: torch.Tensor, gain: torch.Tensor) -> torch.Tensor:
         return x * torch.rsqrt((x * x).mean(-1, keepdim=True) + self.eps) * gain

@@ -141,3 +141,37 @@ def test_the_oracles_choices_are_far_enough_apart(tiny):
     """The comparison of token ids above says something: most of its cases have gaps above twice the tolerance."""
     gaps = [_plain_search(tiny["bf16"], p, 3, 7, None)[1] for p in PROMPTS]
     assert sum(g > 2 * TOL for g in gaps) >= 1, gaps
+
+
+def _walk(rng, groups, beams, prompt, new, page, n_pages):
+    """The forks of a search (as `BeamSearch.search` makes them) with random parents -> the most pages that one of them missed."""
+    from oracle.paged64 import fork_ref
+    width = -(-(prompt + new) // page)
+    tables, lens, refs, worst, _ = fork_ref(np.full((groups, width), -1), np.zeros(groups, int), np.zeros(n_pages, int), range(groups), page, prompt)
+    lens = np.full(groups, prompt)
+    parents = np.arange(groups).repeat(beams)
+    for step in range(new - 1):
+        tables, lens, refs, missing, _ = fork_ref(tables, lens, refs, parents, page, 1)
+        worst, lens = max(worst, missing), lens + 1
+        parents = (rng.integers(0, beams, (groups, beams)) + beams * np.arange(groups)[:, None]).reshape(-1)
+    return worst
+
+
+@pytest.mark.parametrize("groups, beams, prompt, new, page", [(1, 4, 4, 8, 16), (1, 4, 5, 20, 16), (4, 4, 5, 20, 16), (1, 8, 8, 24, 16), (1, 4, 32, 32, 64), (2, 3, 1, 15, 4), (1, 64, 3, 9, 5),
+                                                              (3, 5, 7, 30, 1)])
+def test_the_pool_has_room_for_every_search_that_fits(groups, beams, prompt, new, page):
+    """Pages that beams leave are free only after the step in which others take new ones: the pool holds both."""
+    from cudallm_b200.beam_search import pool_pages
+    for seed in range(30):
+        assert _walk(np.random.default_rng(seed), groups, beams, prompt, new, page, pool_pages(groups * beams, prompt + new, page)) == 0, seed
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beams, prompt, new, page", [(4, 4, 8, 16), (8, 5, 20, 16), (3, 9, 7, 4), (4, 3, 13, 8)])
+def test_searches_that_just_fit(native_lib, tiny, beams, prompt, new, page):
+    """With a cache of exactly the tokens that are asked for, a search finds what it finds with room to spare."""
+    from cudallm_b200.beam_search import BeamSearch
+    tight, roomy = (BeamSearch(tiny["bf16"], rows=2 * beams, max_seq_len=n, page_size=page) for n in (prompt + new, 128))
+    for seed in range(5):
+        prompts = [[int(t) for t in np.random.default_rng([seed, g]).integers(0, 1000, prompt)] for g in range(2)]
+        assert tight.search(prompts, beams=beams, new_tokens=new) == roomy.search(prompts, beams=beams, new_tokens=new)

@@ -4,10 +4,11 @@ A `PagedCache` is a pool of pages for every layer. A sequence is a row of a page
 there is no page) with a length; any number of rows may share pages, counted in `refs` (int32 [pages]). A decode loop
 over beams, per step:
 
-    tables, lens, refs, missing = cache.fork(tables, lens, refs, parents, room=1)   # who continues whom
+    tables, lens, refs, missing = cache.fork(tables, lens, refs, parents.view(-1), room=1)   # who continues whom
     for layer in range(layers):
-        q = cache.append(q, k, v, lens, tables, rope, layer=layer)                  # rotate, store at position lens
-        out = cache.attend(q, tables, lens + 1, layer=layer)
+        turned = cache.append(q, k, v, lens, tables, rope, layer=layer)   # q, k, v of the layer; rotate, store at position lens
+        out = cache.attend(turned, tables, lens + 1, layer=layer)
+    lens = lens + 1                                                       # the token that was stored counts from here on
     scores, parents, tokens = beam_select(logits, scores, keep=beams)
 
 Every call enqueues its work on the current stream of the cache's device, reads lengths, tables and parents there

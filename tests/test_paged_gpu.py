@@ -743,6 +743,29 @@ def test_a_step_in_a_graph():
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
 
 
+def test_the_documented_loop_over_beams():
+    """The loop in the module's documentation, run as it stands for several steps: every row holds its ancestors' keys in order and sees all of them."""
+    loop = "".join(line[4:] for line in paged.__doc__.splitlines(keepends=True) if line.startswith("    "))
+    G, beams, steps, page, vocab = 2, 3, 11, 4, 500
+    cache = _cache(1, 80, 2, page, 64, F16, fill=0.0)
+    tables, lens, refs = cache.rows(G, 8)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    rand = lambda *shape: torch.randn(shape, generator=gen, device="cuda")  # noqa: E731
+    ns = dict(cache=cache, beam_select=paged.beam_select, layers=1, rope=None, beams=beams, tables=tables, lens=lens, refs=refs,
+              parents=_ints([[0] * beams, [1] * beams]), scores=torch.zeros((G, beams), device="cuda"))
+    texts = [[] for _ in range(G)]
+    for step in range(steps):
+        texts = [list(texts[p]) for p in ns["parents"].view(-1).tolist()]
+        ns.update(q=rand(G * beams, 4, 64), k=rand(G * beams, 2, 64).half().float(), v=rand(G * beams, 2, 64).half().float(), logits=rand(G * beams, vocab))
+        exec(compile(loop, "loop", "exec"), ns)
+        assert int(ns["missing"]) == 0 and ns["lens"].tolist() == [step + 1] * (G * beams)
+        for r, text in enumerate(texts):
+            text.append((ns["k"][r], ns["v"][r]))
+            k, v = (_np(torch.stack([t[i] for t in text], 1))[None] for i in range(2))  # one page of all tokens
+            ref, _, size = R.attend64(_np(ns["q"][r:r + 1]), k, v, np.array([[0]]), [len(text)])
+            _within(ns["out"][r:r + 1], ref, ((16 * EPS * np.sqrt(64) * size + 8 * EPS * np.sqrt(len(text))) * np.abs(v).max())[..., None])
+
+
 # ---- refusals ---------------------------------------------------------------------------------
 
 def test_numbers_beyond_32_bits_are_refused():

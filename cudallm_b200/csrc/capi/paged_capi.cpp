@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <numeric>
 #include <string>
 #include <utility>
 
@@ -38,6 +39,49 @@ size_t x_bytes(int x_dtype) { return x_dtype == CUDALLM_X_FP32 ? 4 : 2; }
 bool overlap(const void* p, unsigned long long n, const void* q, unsigned long long m) {
     const auto a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
     return n != 0 && m != 0 && a < b + m && b < a + n;
+}
+
+// Heads of n bytes at p + t * token + h * head, t < tokens.
+struct Heads {
+    const void* p;
+    long long token, head, heads;
+};
+
+// a and b have a byte in common. Exact where their tokens are equally far apart (as they are in a packed projection) and the pairs of heads are few
+// or equally spaced; otherwise only heads that the strides' common divisor keeps apart are known to be.
+bool heads_meet(Heads a, Heads b, long long tokens, long long n) {
+    for (Heads* x : {&a, &b}) {
+        if (tokens == 1) x->token = 0;
+        if (x->heads == 1) x->head = 0;
+    }
+    const long long in_a = (a.heads - 1) * a.head + n, in_b = (b.heads - 1) * b.head + n;  // a token spans
+    if (!overlap(a.p, (tokens - 1) * a.token + in_a, b.p, (tokens - 1) * b.token + in_b)) return false;
+    const long long d = static_cast<long long>(reinterpret_cast<uintptr_t>(b.p)) - static_cast<long long>(reinterpret_cast<uintptr_t>(a.p));
+    if (a.token == b.token) {
+        // [0, n_a) of one token meets [x, x + n_b) of another one (or the same).
+        auto meet = [&](long long x, long long n_a, long long n_b) {
+            if (a.token == 0) return x > -n_b && x < n_a;
+            const long long most = x + (tokens - 1) * a.token, above = most + n_b - 1;  // take tokens off while it stays above -n_b
+            if (above < 0) return false;
+            return most - std::min(above / a.token, 2 * (tokens - 1)) * a.token < n_a;
+        };
+        if (!meet(d, in_a, in_b)) return false;
+        if (a.head == b.head) {
+            for (long long i = 1 - a.heads; i < b.heads; ++i)
+                if (meet(d + i * a.head, n, n)) return true;
+            return false;
+        }
+        if (a.heads * b.heads <= 65536) {
+            for (long long i = 0; i < a.heads; ++i)
+                for (long long j = 0; j < b.heads; ++j)
+                    if (meet(d + j * b.head - i * a.head, n, n)) return true;
+            return false;
+        }
+    }
+    const long long step = std::gcd(std::gcd(a.token, b.token), std::gcd(a.head, b.head));
+    if (step == 0) return true;
+    const long long r = (d % step + step) % step;
+    return r < n || step - r < n;
 }
 
 // Bytes that rows of `width` ints with a stride span.
@@ -141,7 +185,6 @@ int cudallm_paged_append(const cudallm_pages* pages, const cudallm_append_args* 
                      "misaligned pointer");
         CLLM_REQUIRE(a->rotary >= 0 && a->rotary % 2 == 0 && a->rotary <= pages->head_dim, "rotary must be even and at most head_dim");
         CLLM_REQUIRE(a->rotary == 0 || a->inv_freq != nullptr, "inv_freq must be non-null");
-        CLLM_REQUIRE(std::isfinite(a->factor), "factor must be finite");
         CLLM_REQUIRE(a->q == nullptr || (a->n_heads > 0 && a->q_out != nullptr), "q needs n_heads > 0 and q_out");
         CLLM_REQUIRE(a->q_token_stride >= 0 && a->q_head_stride >= 0 && a->k_token_stride >= 0 && a->k_head_stride >= 0 &&
                          a->v_token_stride >= 0 && a->v_head_stride >= 0,
@@ -156,7 +199,13 @@ int cudallm_paged_append(const cudallm_pages* pages, const cudallm_append_args* 
             const unsigned long long in = (T - 1) * a->q_token_stride + (H - 1) * a->q_head_stride + hd;
             const unsigned long long out = (T - 1) * ts + (H - 1) * hs + hd;
             CLLM_REQUIRE(same || !overlap(a->q, es * in, a->q_out, es * out), "q_out must be q or not overlap it");
+            const long long b = es, head = hd * b;
+            const Heads written{a->q_out, ts * b, hs * b, H};
+            CLLM_REQUIRE(!heads_meet(written, {a->k, a->k_token_stride * b, a->k_head_stride * b, pages->n_kv_heads}, T, head) &&
+                             !heads_meet(written, {a->v, a->v_token_stride * b, a->v_head_stride * b, pages->n_kv_heads}, T, head),
+                         "q_out must not overlap k or v");
         }
+        CLLM_REQUIRE(std::isfinite(a->factor), "factor must be finite");
         launch_paged_append(*pages, *a, static_cast<cudaStream_t>(stream));
     });
 }

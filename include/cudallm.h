@@ -305,7 +305,8 @@ unsigned long long cudallm_attend_workspace_bytes(void);
  * sin multiplied by `factor`; the pair is dims (j, j + rotary / 2), or (2j, 2j + 1) with interleaved != 0; dims from
  * `rotary` on are copied. A negative position is padding: q_out is 0 there and nothing is stored; nothing is stored
  * either for a row outside [0, n_rows), a position beyond the table or an entry without a page. Two tokens of one call
- * must not share a slot. rotary 0 stores without rotation. q may be NULL (keys and values only). */
+ * must not share a slot. rotary 0 stores without rotation. q may be NULL (keys and values only). q_out must not overlap k
+ * or v (heads of one packed projection may lie between each other), nor q, k and v the pages. */
 typedef struct {
     int struct_size; /* sizeof(cudallm_append_args) */
     int layer, x_dtype, n_tokens, n_heads, n_rows, table_width, rotary, interleaved;

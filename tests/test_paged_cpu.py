@@ -94,6 +94,37 @@ def test_append_refusals(native_lib, over):
     assert _refused(native_lib, "cudallm_paged_append", _pages(), _append(**over))
 
 
+def test_append_refuses_outputs_over_the_keys_or_values(native_lib):
+    """Layouts of q_out, k and v around each other, in one buffer: refused exactly where a head of q_out shares a byte with a head of k or v, for equal
+    token strides; for others wherever they share one. (factor is not a number, so that every call is refused by one check or the other.)"""
+    rng = np.random.default_rng(0)
+    counts = {True: 0, False: 0}
+    for i in range(6000):
+        T, H, KV, hd = int(rng.integers(1, 5)), int(rng.integers(1, 4)), int(rng.integers(1, 4)), 8
+        hs = [int(rng.choice([8, 9, 12, 16, 24, 40, 41])) for _ in range(3)]
+        ts = [int(rng.choice([8, 24, 33, 48, 64, 72, 100, 120]))] * 3 if i % 3 else [int(rng.choice([24, 48, 64, 100])) for _ in range(3)]
+        if i % 5 == 0:
+            hs = [hs[0]] * 3
+        at = [0, *(int(rng.integers(-200, 200)) for _ in range(2))]
+        base = FAKE + 4096
+        assert _refused(native_lib, "cudallm_paged_append", _pages(n_kv_heads=KV, head_dim=hd, page_size=1, token_stride=8, head_stride=8, page_stride=KV * 8, layer_stride=KV * 64),
+                        _append(n_tokens=T, n_rows=T, n_heads=H, rotary=8, factor=float("nan"), q=4 * FAKE, q_token_stride=64, q_head_stride=8,
+                                q_out=base, out_token_stride=ts[0], out_head_stride=hs[0], k=base + 4 * at[1], k_token_stride=ts[1], k_head_stride=hs[1],
+                                v=base + 4 * at[2], v_token_stride=ts[2], v_head_stride=hs[2]))
+        message = native_lib.cudallm_last_error()
+        sets = [{a + t * x + h * y + e for t in range(T) for h in range(n) for e in range(hd)} for a, x, y, n in zip(at, ts, hs, (H, KV, KV))]
+        meets = bool(sets[0] & sets[1] or sets[0] & sets[2])
+        if b"heads of q_out must not overlap" in message:
+            continue
+        refused = b"must not overlap k or v" in message
+        assert refused or b"factor" in message, message
+        assert refused or not meets, (T, H, KV, hs, ts, at)
+        if len(set(ts)) == 1:
+            assert refused == meets, (T, H, KV, hs, ts, at)
+            counts[meets] += 1
+    assert min(counts.values()) > 300, counts
+
+
 @pytest.mark.parametrize("over", [dict(struct_size=0), dict(n_rows=-1), dict(n_out=65537), dict(room=-1), dict(tables=None), dict(lens=None), dict(refs=None),
                                   dict(parents=None), dict(tables_out=FAKE), dict(tables_out=FAKE + 20), dict(refs_out=3 * FAKE), dict(missing=3 * FAKE + 28),
                                   dict(lens_out=5 * FAKE + 4), dict(missing=None), dict(workspace_bytes=0), dict(table_out_stride=1)], ids=str)

@@ -380,6 +380,26 @@ def test_append_strides_and_in_place(dim, offset, stride):
     _check_append(cache, None, k, v, list(range(n)), table, rope, rows=rows)
 
 
+@pytest.mark.parametrize("layout", ["token", "head", "each"])
+def test_append_in_place_in_a_packed_projection(layout):
+    """q, k and v of one buffer (heads side by side in a token, tokens in a head, or q, k and v of each head together), q turned in place."""
+    n, heads = 21, 3
+    table, pages = _layout([n], 8)
+    cache = _cache(1, pages, heads, 8, 64, F16)
+    if layout == "token":
+        q, k, v = torch.randn((n, 3 * heads, 64), device="cuda", dtype=F16).split(heads, 1)
+    elif layout == "head":
+        q, k, v = torch.randn((3 * heads, n, 64), device="cuda", dtype=F16).transpose(0, 1).split(heads, 1)
+    else:
+        q, k, v = torch.randn((n, heads, 3 * 64), device="cuda", dtype=F16).split(64, 2)
+    k0, v0 = k.clone(), v.clone()
+    _check_append(cache, q, k, v, list(range(n)), table, paged.Rope.make(64), rows=[0] * n, out=q)
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+    for out in (k, v):
+        with pytest.raises(CudaLLMError, match="overlap k or v"):
+            cache.append(q.clone(), k, v, _ints(range(n)), _ints(table), None, rows=_ints([0] * n), out=out)
+
+
 def test_append_one_token_a_row_padding_and_places_outside():
     table, pages = _layout([64] * 6, 16)
     table[2, 1] = -1

@@ -196,11 +196,9 @@ int cudallm_paged_append(const cudallm_pages* pages, const cudallm_append_args* 
             const bool head_outer = (T == 1 || ts >= hd) && (H == 1 || hs >= (T == 1 ? hd : ts * (T - 1) + hd));
             CLLM_REQUIRE(token_outer || head_outer, "heads of q_out must not overlap");
             const bool same = a->q_out == a->q && (T == 1 || ts == a->q_token_stride) && (H == 1 || hs == a->q_head_stride);
-            const unsigned long long in = (T - 1) * a->q_token_stride + (H - 1) * a->q_head_stride + hd;
-            const unsigned long long out = (T - 1) * ts + (H - 1) * hs + hd;
-            CLLM_REQUIRE(same || !overlap(a->q, es * in, a->q_out, es * out), "q_out must be q or not overlap it");
             const long long b = es, head = hd * b;
             const Heads written{a->q_out, ts * b, hs * b, H};
+            CLLM_REQUIRE(same || !heads_meet(written, {a->q, a->q_token_stride * b, a->q_head_stride * b, H}, T, head), "q_out must be q or not overlap it");
             CLLM_REQUIRE(!heads_meet(written, {a->k, a->k_token_stride * b, a->k_head_stride * b, pages->n_kv_heads}, T, head) &&
                              !heads_meet(written, {a->v, a->v_token_stride * b, a->v_head_stride * b, pages->n_kv_heads}, T, head),
                          "q_out must not overlap k or v");

@@ -400,6 +400,17 @@ def test_append_in_place_in_a_packed_projection(layout):
             cache.append(q.clone(), k, v, _ints(range(n)), _ints(table), None, rows=_ints([0] * n), out=out)
 
 
+def test_append_output_between_the_queries():
+    """A buffer whose tokens hold q, k, v and a place for the turned q: nothing of it overlaps."""
+    n, heads = 21, 3
+    table, pages = _layout([n], 8)
+    cache = _cache(1, pages, heads, 8, 64, F16)
+    q, k, v, out = torch.randn((n, 4 * heads, 64), device="cuda", dtype=F16).split(heads, 1)
+    q0 = q.clone()
+    _check_append(cache, q, k, v, list(range(n)), table, paged.Rope.make(64), rows=[0] * n, out=out)
+    assert torch.equal(q, q0)
+
+
 def test_append_one_token_a_row_padding_and_places_outside():
     table, pages = _layout([64] * 6, 16)
     table[2, 1] = -1

@@ -71,9 +71,10 @@ def _beam_calls():
 
 
 def _beam_args():
-    """This thread's argument struct of beam_select."""
+    """This thread's argument struct of beam_select, its reference, and this thread's workspaces by device: two launches make up a call, and those
+    of two threads on one stream may come in between each other."""
     if not hasattr(_beam, "args"):
-        _beam.args = _args("cudallm_beam_args")
+        _beam.args = (*_args("cudallm_beam_args"), {})
     return _beam.args
 
 
@@ -97,9 +98,6 @@ class _Workspaces:
         if w is None or w.numel() < size:
             w = self.by_stream[stream] = self._new(size)
         return w
-
-
-_shared: dict[int, _Workspaces] = {}
 
 
 class _OnDevice:
@@ -381,7 +379,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     """The `keep` best continuations of each group of beams: logits [groups * beams][vocab] (fp32, fp16 or bf16), scores fp32
     [groups][beams] (the beams' log-probabilities so far), finished int32 [groups][beams] (a beam with a nonzero value only
     continues with `eos`, at its score). Returns (scores fp32, parents int32, tokens int32), each [groups][keep], best
-    first; parents are rows of logits, as PagedCache.fork takes them. Equal candidates go to the lower row, then token."""
+    first; parents are rows of logits, as PagedCache.fork takes them (flattened). Equal candidates go to the lower row, then
+    token. Any thread may call it."""
     x = _X.get(logits.dtype)
     if x is None or logits.dim() != 2 or not logits.is_cuda:
         _refuse("logits must be an fp32, fp16 or bf16 tensor [groups * beams][vocab] on the GPU")
@@ -395,7 +394,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
         _refuse("logits must have groups * beams rows with their values side by side")
     if not (1 <= keep <= _INT_MAX and 0 <= eos <= _INT_MAX):
         _refuse("keep must be positive, eos a token")
-    a, ref = _beam_args()
+    a, ref, spaces_of = _beam_args()
     a.finished = None if finished is None else _int32(finished, dev, (groups, beams), "finished")
     if out is None:
         best = scores.new_empty(groups, keep)
@@ -414,9 +413,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     select, size = _beam_calls()
     index = dev.index
     stream = _stream_of(index)
-    spaces = _shared.get(index)
+    spaces = spaces_of.get(index)
     if spaces is None:
-        spaces = _shared[index] = _Workspaces(dev, _BEAM_COUNTERS)
+        spaces = spaces_of[index] = _Workspaces(dev, _BEAM_COUNTERS)
     w = spaces.get(stream, size(rows, vocab, keep))
     a.workspace, a.workspace_bytes = w.data_ptr(), w.numel()
     if _current_device() == index:

@@ -251,8 +251,8 @@ int cudallm_attention_noalloc(const float* q, const unsigned short* k_cache, con
  * so no content of those arrays leads to an access outside of the caller's buffers.
  *
  * Workspaces: `workspace` points to at least cudallm_*_workspace_bytes() bytes, 256-byte aligned; its contents do not matter (but for
- * cudallm_beam_select's, see there). One may serve the cudallm_paged_* calls one after the other on one stream; calls that may overlap (other
- * streams) need their own. */
+ * cudallm_beam_select's, see there). One may serve the cudallm_paged_* calls one after the other on one stream; calls that may overlap (on
+ * other streams, or from other host threads: a call may be two launches) need their own. */
 
 #define CUDALLM_BEAM_COUNTER_BYTES 16384
 

@@ -10,6 +10,8 @@ each plus half a unit in the last place of the output's type (2^-11 fp16, 2^-8 b
 exactly."""
 from __future__ import annotations
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -772,6 +774,45 @@ def test_a_step_in_a_graph():
         want = step(other)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
+
+
+def test_beam_workspaces_of_threads(monkeypatch):
+    """Threads that call on one stream each bring a workspace of their own. Nothing is launched here: the calls only show what they would pass."""
+    seen, both = [], threading.Barrier(2)
+    select, size = paged._beam_calls()
+    monkeypatch.setattr(paged, "_beam_calls", lambda: (lambda ref, stream: seen.append((ref._obj.workspace, stream)) or 0, size))
+    x, s = torch.zeros((64, 128256), device="cuda"), torch.zeros((8, 8), device="cuda")
+
+    def call():
+        both.wait()
+        paged.beam_select(x, s, keep=8)
+        both.wait()  # neither is over before the other has called
+
+    paged.beam_select(x, s, keep=8)  # this thread's
+    threads = [threading.Thread(target=call) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(seen) == 3 and len({stream for _, stream in seen}) == 1 and len({workspace for workspace, _ in seen}) == 3
+
+
+def test_beam_from_several_threads():
+    """Four threads select from logits of their own on one stream, in the form of two launches; each gets what it gets alone."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    xs = [torch.randn((64, 128256), generator=gen, device="cuda") for _ in range(4)]
+    s = torch.zeros((8, 8), device="cuda")
+    refs = [paged.beam_select(x, s, keep=8) for x in xs]
+    torch.cuda.synchronize()
+    found = [[] for _ in xs]
+    threads = [threading.Thread(target=lambda i=i: found[i].extend(paged.beam_select(xs[i], s, keep=8) for _ in range(100))) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for got, ref in zip(found, refs):
+        assert len(got) == 100 and all(torch.equal(a, b) for g in got for a, b in zip(g, ref))
 
 
 def test_the_documented_loop_over_beams():

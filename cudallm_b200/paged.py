@@ -91,8 +91,15 @@ class _Workspaces:
             w[:self.counters].zero_()
         return w
 
+    def _capturing(self) -> bool:
+        """Whether this device's current stream is being captured (torch answers for the current device)."""
+        if _current_device() == self.device.index:
+            return torch.cuda.is_current_stream_capturing()
+        with _OnDevice(self.device.index):
+            return torch.cuda.is_current_stream_capturing()
+
     def get(self, stream: int, size: int) -> torch.Tensor:
-        if torch.cuda.is_current_stream_capturing():  # the graph's own, which later calls must not replace
+        if self._capturing():  # the graph's own, which later calls must not replace
             return self._new(size)
         w = self.by_stream.get(stream)
         if w is None or w.numel() < size:

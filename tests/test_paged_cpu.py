@@ -154,6 +154,24 @@ def test_messages_and_workspace_sizes(native_lib):
     assert native_lib.cudallm_beam_workspace_bytes(64, 128256, 16) > 64 * 16 * 8 and native_lib.cudallm_beam_workspace_bytes(4, 100, 65) == 0
 
 
+def test_a_graph_keeps_its_workspace_whichever_device_is_current(monkeypatch):
+    """Calls for device 1 while its stream is captured and device 0 is current: each workspace is the graph's own. Otherwise the stream's is kept."""
+    now, capturing = [0], [1]
+    monkeypatch.setattr(paged, "_current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[0])
+    monkeypatch.setattr(torch.cuda, "set_device", lambda i: now.__setitem__(0, i))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now[0] in capturing)
+    monkeypatch.setattr(paged._Workspaces, "_new", lambda self, size: torch.empty(size, dtype=torch.uint8))
+    spaces = paged._Workspaces(torch.device("cuda", 1))
+    for current in (0, 1):
+        now[0] = current
+        a, b = spaces.get(7, 100), spaces.get(7, 100)
+        assert a is not b and not spaces.by_stream and now[0] == current
+    capturing[0] = 0  # a capture on another device does not matter
+    a = spaces.get(7, 100)
+    assert a is spaces.get(7, 100) and spaces.by_stream[7] is a
+
+
 def test_tensors_off_the_gpu_are_refused():
     k = torch.zeros((1, 2, 1, 8, 64), dtype=torch.float16)
     with pytest.raises(paged.CudaLLMError):

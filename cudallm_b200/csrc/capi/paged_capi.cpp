@@ -41,6 +41,14 @@ bool overlap(const void* p, unsigned long long n, const void* q, unsigned long l
     return n != 0 && m != 0 && a < b + m && b < a + n;
 }
 
+// [q, q + m) and one of the rows [p + r * stride, + n) share a byte.
+bool rows_meet(const void* p, long long rows, long long n, long long stride, const void* q, long long m) {
+    if (!overlap(p, (rows - 1) * stride + n, q, m)) return false;
+    if (rows == 1 || stride == 0) return true;
+    const long long d = static_cast<long long>(reinterpret_cast<uintptr_t>(q)) - static_cast<long long>(reinterpret_cast<uintptr_t>(p));
+    return std::min((d + m - 1) / stride, rows - 1) * stride + n > d;  // the last row that starts before the end of q
+}
+
 // Heads of n bytes at p + t * token + h * head, t < tokens.
 struct Heads {
     const void* p;
@@ -285,6 +293,16 @@ int cudallm_beam_select(const cudallm_beam_args* a, void* stream) {
                      "misaligned pointer");
         CLLM_REQUIRE(rows == 1 || a->row_stride >= a->vocab || a->row_stride == 0, "row_stride must be at least vocab, or 0 for one shared row");
         CLLM_REQUIRE(a->finished == nullptr || (a->eos >= 0 && a->eos < a->vocab), "eos must be in [0, vocab)");
+        const long long outs = 4LL * a->n_groups * a->keep;
+        const std::array<const void*, 3> out{a->out_scores, a->out_parents, a->out_tokens};
+        for (size_t o = 0; o < out.size(); ++o) {
+            // A group's scores are read before its own are written, so that they may be written in place where each has as many.
+            const bool in_place = o == 0 && a->out_scores == a->scores && a->keep == a->beams;
+            CLLM_REQUIRE((in_place || !overlap(a->scores, 4ull * rows, out[o], outs)) && (a->finished == nullptr || !overlap(a->finished, 4ull * rows, out[o], outs)) &&
+                             !rows_meet(a->logits, rows, es * a->vocab, es * a->row_stride, out[o], outs),
+                         "outputs must not overlap inputs (but out_scores may be scores where keep is beams)");
+            for (size_t k = 0; k < o; ++k) CLLM_REQUIRE(!overlap(out[k], outs, out[o], outs), "outputs must not overlap each other");
+        }
         check_workspace(a->workspace, a->workspace_bytes, beam_workspace_bytes(rows, a->vocab, a->keep));
         launch_beam_select(*a, static_cast<cudaStream_t>(stream));
     });

@@ -382,7 +382,8 @@ unsigned long long cudallm_pages_workspace_bytes(int n_pages, int rows);
  * w of logits, or, where finished[g][w] != 0 (finished may be NULL), x = 0 at eos and -inf elsewhere. A candidate that
  * is not a number counts as -inf. The `keep` best of each group, in order: larger candidate, then lower beam, then
  * larger logit (one that is not a number: -inf), then lower token. out_parents are rows of logits (as
- * cudallm_paged_fork takes them). beams 1 .. 64, keep 1 .. 64 and at most beams * vocab, vocab at most 2^24. */
+ * cudallm_paged_fork takes them). beams 1 .. 64, keep 1 .. 64 and at most beams * vocab, vocab at most 2^24. Outputs
+ * must not overlap inputs or each other, but out_scores may be scores where keep equals beams. */
 typedef struct {
     int struct_size; /* sizeof(cudallm_beam_args) */
     int x_dtype, n_groups, beams, keep, vocab, eos, reserved;

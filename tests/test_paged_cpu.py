@@ -145,6 +145,26 @@ def test_beam_refusals(native_lib, over):
     assert _refused(native_lib, "cudallm_beam_select", _beam(**over))
 
 
+APART = dict(logits=FAKE, scores=2 * FAKE, finished=3 * FAKE, out_scores=4 * FAKE, out_parents=5 * FAKE, out_tokens=6 * FAKE, workspace=7 * FAKE)
+
+
+@pytest.mark.parametrize("over", [dict(out_scores=2 * FAKE + 4), dict(out_scores=2 * FAKE, keep=5), dict(out_scores=2 * FAKE, keep=3), dict(out_parents=2 * FAKE), dict(out_tokens=2 * FAKE + 28),
+                                  dict(out_parents=3 * FAKE - 28), dict(out_tokens=FAKE + 400), dict(out_scores=FAKE + 3196), dict(out_tokens=5 * FAKE + 16), dict(out_parents=4 * FAKE),
+                                  dict(row_stride=107, out_parents=FAKE + 400), dict(row_stride=108, out_parents=FAKE + 432 * 7 + 396), dict(row_stride=0, out_scores=FAKE + 396)],
+                         ids=str)
+def test_beam_refuses_overlaps(native_lib, over):
+    assert _refused(native_lib, "cudallm_beam_select", _beam(**{**APART, **over}))
+    assert b"overlap" in native_lib.cudallm_last_error()
+
+
+@pytest.mark.parametrize("over", [dict(), dict(out_scores=2 * FAKE), dict(out_scores=2 * FAKE + 32), dict(out_scores=FAKE + 3200), dict(row_stride=108, out_parents=FAKE + 400),
+                                  dict(row_stride=108, out_parents=FAKE + 432 * 7 + 400), dict(row_stride=0, out_scores=FAKE + 400), dict(finished=None, out_tokens=3 * FAKE)], ids=str)
+def test_beam_takes_what_lies_apart(native_lib, over):
+    """The workspace is too small, so that these are refused as well, after the check for overlaps."""
+    assert _refused(native_lib, "cudallm_beam_select", _beam(**{**APART, **over, "workspace_bytes": 8}))
+    assert b"workspace" in native_lib.cudallm_last_error()
+
+
 def test_messages_and_workspace_sizes(native_lib):
     assert _refused(native_lib, "cudallm_paged_attend", _pages(), _attend(layer=7))
     assert b"layer" in native_lib.cudallm_last_error()

@@ -717,6 +717,16 @@ def test_beam_strided_and_shared_rows():
     _check_beam(wide[:1].expand(4, 1101), [[-1.0, -1.5, -2.0, -2.5]], 8)
 
 
+@pytest.mark.parametrize("groups, vocab", [(3, 5000), (20, 128256)])
+def test_beam_scores_in_place(groups, vocab):
+    """One launch and two: the new scores written over the old ones, as many of them."""
+    x, s = torch.randn((groups * 4, vocab), device="cuda"), _f32(np.random.default_rng(6).normal(-5, 1, (groups, 4)))
+    ref = paged.beam_select(x, s, keep=4)
+    out = (s, *(torch.empty_like(ref[1]) for _ in range(2)))
+    got = paged.beam_select(x, s, keep=4, out=out)
+    assert got is out and all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
 def test_beam_same_bits_in_a_graph_and_on_two_streams():
     x, s = torch.randn((16, 128256), device="cuda"), _f32(np.random.default_rng(2).normal(-5, 1, (4, 4)))
     ref = paged.beam_select(x, s, keep=8)

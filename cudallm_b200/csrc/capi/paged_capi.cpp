@@ -170,7 +170,13 @@ int cudallm_paged_attend(const cudallm_pages* pages, const cudallm_attend_args* 
         CLLM_REQUIRE(aligned(a->q, es) && aligned(a->out, es) && aligned(a->lens, 4) && aligned(a->lse, 4), "misaligned pointer");
         CLLM_REQUIRE(a->q_seq_stride >= 0 && a->q_head_stride >= 0, "q strides must not be negative");
         const unsigned long long span = (a->n_seq - 1) * a->q_seq_stride + (a->n_heads - 1) * a->q_head_stride + pages->head_dim;
-        CLLM_REQUIRE(!overlap(a->q, es * span, a->out, es * a->n_seq * a->n_heads * pages->head_dim), "out must not overlap q");
+        const unsigned long long heads = static_cast<unsigned long long>(a->n_seq) * a->n_heads, outs = es * heads * pages->head_dim;
+        const unsigned long long lses = a->lse != nullptr ? 4 * heads : 0, table = table_bytes(a->n_seq, a->table_width, a->table_stride);
+        CLLM_REQUIRE(!overlap(a->q, es * span, a->out, outs), "out must not overlap q");
+        CLLM_REQUIRE(!overlap(a->tables, table, a->out, outs) && !overlap(a->lens, 4ull * a->n_seq, a->out, outs), "out must not overlap tables or lens");
+        CLLM_REQUIRE(!overlap(a->q, es * span, a->lse, lses) && !overlap(a->out, outs, a->lse, lses) && !overlap(a->tables, table, a->lse, lses) &&
+                         !overlap(a->lens, 4ull * a->n_seq, a->lse, lses),
+                     "lse must not overlap q, out, tables or lens");
         check_workspace(a->workspace, a->workspace_bytes, attend_workspace_bytes());
         launch_paged_attend(*pages, *a, static_cast<cudaStream_t>(stream));
     });
@@ -204,6 +210,11 @@ int cudallm_paged_append(const cudallm_pages* pages, const cudallm_append_args* 
             const bool head_outer = (T == 1 || ts >= hd) && (H == 1 || hs >= (T == 1 ? hd : ts * (T - 1) + hd));
             CLLM_REQUIRE(token_outer || head_outer, "heads of q_out must not overlap");
             const bool same = a->q_out == a->q && (T == 1 || ts == a->q_token_stride) && (H == 1 || hs == a->q_head_stride);
+            const unsigned long long span = es * ((T - 1) * (T > 1 ? ts : 0) + (H - 1) * (H > 1 ? hs : 0) + hd);
+            CLLM_REQUIRE(!overlap(a->positions, 4ull * T, a->q_out, span) && (a->rows == nullptr || !overlap(a->rows, 4ull * T, a->q_out, span)) &&
+                             !overlap(a->tables, table_bytes(a->n_rows, a->table_width, a->table_stride), a->q_out, span) &&
+                             !overlap(a->inv_freq, 2ull * a->rotary, a->q_out, span),
+                         "q_out must not overlap positions, rows, tables or inv_freq");
             const long long b = es, head = hd * b;
             const Heads written{a->q_out, ts * b, hs * b, H};
             CLLM_REQUIRE(same || !heads_meet(written, {a->q, a->q_token_stride * b, a->q_head_stride * b, H}, T, head), "q_out must be q or not overlap it");

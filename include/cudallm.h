@@ -278,8 +278,8 @@ typedef struct {
  * clamped to it) whose page exists; n_heads / n_kv_heads query heads share a key head. lse (or NULL): the natural
  * logarithm of the sum of the exponentials. No position left: out 0, lse -inf; a score that is not a number: out and
  * lse of its head are not numbers either. Scores, statistics and sums are fp32.
- * q [n_seq][n_heads][head_dim] has its own strides, out and lse are contiguous; out has q's type and must not
- * overlap q. Values in unused slots of a page do not matter; keys and values of used ones must be finite. */
+ * q [n_seq][n_heads][head_dim] has its own strides, out and lse are contiguous; out has q's type; out and
+ * lse must not overlap the inputs or each other. Values in unused slots of a page do not matter; keys and values of used ones must be finite. */
 typedef struct {
     int struct_size; /* sizeof(cudallm_attend_args) */
     int layer, x_dtype, n_seq, n_heads, table_width, window;
@@ -305,8 +305,8 @@ unsigned long long cudallm_attend_workspace_bytes(void);
  * sin multiplied by `factor`; the pair is dims (j, j + rotary / 2), or (2j, 2j + 1) with interleaved != 0; dims from
  * `rotary` on are copied. A negative position is padding: q_out is 0 there and nothing is stored; nothing is stored
  * either for a row outside [0, n_rows), a position beyond the table or an entry without a page. Two tokens of one call
- * must not share a slot. rotary 0 stores without rotation. q may be NULL (keys and values only). q_out must not overlap k
- * or v (heads of one packed projection may lie between each other), nor q, k and v the pages. */
+ * must not share a slot. rotary 0 stores without rotation. q may be NULL (keys and values only). q_out must not overlap any
+ * other input (heads of one packed projection may lie between each other), nor q, k and v the pages. */
 typedef struct {
     int struct_size; /* sizeof(cudallm_append_args) */
     int layer, x_dtype, n_tokens, n_heads, n_rows, table_width, rotary, interleaved;

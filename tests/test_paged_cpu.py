@@ -94,6 +94,26 @@ def test_append_refusals(native_lib, over):
     assert _refused(native_lib, "cudallm_paged_append", _pages(), _append(**over))
 
 
+@pytest.mark.parametrize("over", [dict(out=6 * FAKE - 2044), dict(out=6 * FAKE), dict(out=5 * FAKE + 20), dict(lse=FAKE + 2044), dict(lse=2 * FAKE), dict(lse=5 * FAKE - 28), dict(lse=6 * FAKE + 4),
+                                  dict(lse=2 * FAKE + 2044)], ids=str)
+def test_attend_refuses_outputs_over_inputs_or_each_other(native_lib, over):
+    apart = dict(q=FAKE, out=2 * FAKE, lse=3 * FAKE, tables=5 * FAKE, lens=6 * FAKE)
+    assert _refused(native_lib, "cudallm_paged_attend", _pages(), _attend(**{**apart, **over}))
+    assert b"overlap" in native_lib.cudallm_last_error()
+    assert _refused(native_lib, "cudallm_paged_attend", _pages(), _attend(**apart, workspace_bytes=8))  # as they are, only the workspace is refused
+    assert b"workspace" in native_lib.cudallm_last_error()
+
+
+@pytest.mark.parametrize("over", [dict(positions=2 * FAKE + 2044), dict(rows=2 * FAKE - 4), dict(tables=2 * FAKE + 1024), dict(inv_freq=2 * FAKE - 124)], ids=str)
+def test_append_refuses_outputs_over_indexes(native_lib, over):
+    apart = dict(q=FAKE, q_out=2 * FAKE, k=3 * FAKE, v=4 * FAKE, positions=5 * FAKE, rows=6 * FAKE, tables=7 * FAKE, inv_freq=8 * FAKE, factor=float("nan"), k_token_stride=128,
+                 k_head_stride=64, v_token_stride=128, v_head_stride=64)
+    assert _refused(native_lib, "cudallm_paged_append", _pages(), _append(**{**apart, **over}))
+    assert b"overlap" in native_lib.cudallm_last_error()
+    assert _refused(native_lib, "cudallm_paged_append", _pages(), _append(**apart))
+    assert b"factor" in native_lib.cudallm_last_error()
+
+
 def test_append_refuses_outputs_over_the_keys_or_values(native_lib):
     """Layouts of q_out, k and v around each other, in one buffer: refused exactly where a head of q_out shares a byte with a head of k or v, for equal
     token strides; for others wherever they share one. (factor is not a number, so that every call is refused by one check or the other.)"""

@@ -136,6 +136,8 @@ def _table(t: torch.Tensor, device: torch.device, name: str) -> tuple[int, int, 
     if t.dtype is not torch.int32 or t.get_device() != device.index or t.dim() != 2:
         _refuse(f"{name} must be an int32 tensor [rows][width] on {device}")
     rows, width = t.shape
+    if rows | width > _INT_MAX:  # all ones below 2^31: either of them is
+        _refuse(f"{name} must have fewer than 2^31 rows and entries a row")
     stride, inner = t.stride()
     if inner != 1 and rows and width > 1:
         _refuse(f"{name} must have its entries side by side")
@@ -147,6 +149,8 @@ def _heads(t: torch.Tensor, device: torch.device, dtype: torch.dtype, dim: int, 
     if t.dtype is not dtype or t.get_device() != device.index or t.dim() != 3:
         _refuse(f"{name} must be a {dtype} tensor [tokens][heads][{dim}] on {device}, got {t.dtype} {list(t.shape)} on {t.device}")
     n, heads, d = t.shape
+    if n | heads > _INT_MAX:
+        _refuse(f"{name} must have fewer than 2^31 tokens and heads")
     ts, hs, inner = t.stride()
     if d != dim or (inner != 1 and n and heads):
         _refuse(f"{name} must be [tokens][heads][{dim}] with its dims side by side, got {list(t.shape)} with strides {list(t.stride())}")
@@ -335,6 +339,8 @@ class PagedCache:
         if parents.dim() != 1 or not 0 <= room <= _INT_MAX:
             _refuse("parents must be a vector, room not negative and below 2^31")
         n_out = parents.shape[0]
+        if n_out > _INT_MAX:
+            _refuse("parents must have fewer than 2^31 entries")
         a.lens = _int32(lens, dev, (n_rows,), "lens")
         a.refs = _int32(refs, dev, (self.n_pages,), "refs")
         a.parents = _int32(parents, dev, (n_out,), "parents")
@@ -399,8 +405,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, keep: int, finish
     row_stride, inner = logits.stride()
     if rows != groups * beams or (rows and vocab > 1 and inner != 1):
         _refuse("logits must have groups * beams rows with their values side by side")
-    if not (1 <= keep <= _INT_MAX and 0 <= eos <= _INT_MAX):
-        _refuse("keep must be positive, eos a token")
+    if not (1 <= keep <= _INT_MAX and 0 <= eos <= _INT_MAX and rows | vocab <= _INT_MAX):
+        _refuse("keep must be positive, eos a token, and sizes below 2^31")
     a, ref, spaces_of = _beam_args()
     a.finished = None if finished is None else _int32(finished, dev, (groups, beams), "finished")
     if out is None:

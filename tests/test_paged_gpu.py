@@ -864,6 +864,19 @@ def test_numbers_beyond_32_bits_are_refused():
         assert e.value.code == 1
 
 
+def test_sizes_beyond_32_bits_are_refused():
+    """Neither may a tensor's sizes come out as others: a row of 2^32 + 5 logits is not one of 5."""
+    cache = _cache(2, 8, 2, 16, 64, F16)
+    t, n, r = cache.rows(2, 3)
+    q = torch.zeros((1, 1, 64), device="cuda")
+    logits = torch.empty((1, 2 ** 32 + 5), dtype=F16, device="cuda")
+    for call in (lambda: paged.beam_select(logits, _f32([[0.0]]), keep=2), lambda: cache.attend(q.expand(1, 2 ** 32 + 4, 64), t[:1], n[:1]),
+                 lambda: cache.compact(t.new_empty((0, 2 ** 32 + 3)), r), lambda: cache.fork(t.new_empty((0, 2 ** 32 + 3)), n[:0], r, n[:0])):
+        with pytest.raises(CudaLLMError) as e:
+            call()
+        assert e.value.code == 1
+
+
 def test_refusals():
     cache = _cache(2, 8, 2, 16, 64, F16)
     t, n, r = cache.rows(2, 3)

@@ -175,3 +175,14 @@ def test_searches_that_just_fit(native_lib, tiny, beams, prompt, new, page):
     for seed in range(5):
         prompts = [[int(t) for t in np.random.default_rng([seed, g]).integers(0, 1000, prompt)] for g in range(2)]
         assert tight.search(prompts, beams=beams, new_tokens=new) == roomy.search(prompts, beams=beams, new_tokens=new)
+
+
+CASES = next(m for m in test_against_a_plain_search.pytestmark if m.name == "parametrize").args[1]
+
+
+@pytest.mark.parametrize("dtype, beams, page, eos", CASES)
+def test_every_comparison_reaches_the_token_ids(tiny, dtype, beams, page, eos):
+    """In each case of the comparison with a plain search, the token ids of one prompt or more are compared (its gap is above twice the tolerance)."""
+    if eos is not None:
+        eos = _plain_search(tiny[dtype], PROMPTS[0], beams, 2, None)[0][1][1][0]
+    assert any(_plain_search(tiny[dtype], p, beams, 7, eos)[1] > 2 * TOL for p in PROMPTS)

@@ -5,16 +5,19 @@
 // Within a row candidates rank as (logit, then lower token), so the `keep` best by logit of each chunk of a row are the
 // only ones that can be among the group's.
 //
-// chunk stage: one block per 8192 logits, which stay in registers (one read of the logits, what bounds the operator at
-//   many rows). It leaves their maximum, their sum of exponentials and the sorted keys of their `keep` best. The maxima of 512
-//   pieces give a lower bound of the keep-th best; the few logits above it are ranked by counting. Where more than 256 are above it (ties, a masked vocabulary) the keep-th key itself is
-//   searched bit by bit over value and token.
+// chunk stage: one block per 8192 logits, which stay in registers (one read of the logits). It leaves their maximum, their sum of exponentials and the
+//   sorted keys of their `keep` best. The maxima of 512 pieces give a lower bound of the keep-th best; the few logits above it are ranked by
+//   counting. Where more than 256 are above it (ties, a masked vocabulary) the keep-th key itself is searched bit by bit over value and token.
 // group stage: joins the rows' sums and ranks the lists' candidates in the same way. Up to 512 chunks the last block of a
 //   group to finish does it; with more, a block for each group in a second launch, in place when the chunks are done (us a call with one
-//   launch and with two: 4 rows x 128256 12.8 and 15.4, 32 rows 13.0 and 15.3, 64 rows 17.4 and 15.3).
+//   launch and with two, at 128256 tokens: 4 rows 12.8 and 15.4, 32 rows 13.0 and 15.3, 64 rows 17.4 and 15.3).
 //
-// Measured (B200, graph replay): 64 rows x 128256, fp32, 22.9 us (1.4 TB/s; the instructions of a list, about 40 a logit and warp, bound it), bf16
-// with 40 rows finished 15.6 us; 4 rows 12.2 us.
+// Latency bounds it, not the read: a chunk is a chain of load, maximum, bound, list and rank. 64 rows x 128256 fp32 (8 x 8 beams, keep 8; ncu, cold
+// caches): chunks 17 us at 1.9 TB/s, 1024 blocks in 1.7 waves of four an SM (64 registers), 40 % of the issue slots, a third of a warp's time
+// waiting for its logits; groups 10 us on 8 blocks, of which half waits at barriers for keys from L2.
+//
+// Measured (B200, graph replay, other logits each time): 64 rows x 128256, fp32, 20.5 us (keep 8), 22.3 (16), 31.6 (64); bf16 the same; with 40 rows
+// finished, keep 16, 15.6 us; 16 rows 12.3 us; 4 rows 12.0 us; 64 rows x 32000 12.4 us.
 #include <cmath>
 
 #include "common/check.h"

@@ -5,7 +5,8 @@
 // Every input is read once and every output written once: HBM bounds it at many tokens, launch latency at few. A block
 // takes one or more tokens, computes their cosines once for all heads, and its threads walk the heads in units of 8
 // dims (16-byte accesses of 16-bit types): the two halves of 8 pairs, 4 interleaved pairs, or 8 dims that are copied.
-// Where strides or sizes do not allow that, a unit is one pair or one dim.
+// Where strides or sizes do not allow that, a unit is one pair or one dim, and the number of loads bounds it (16383 tokens of 48 heads x 128, bf16:
+// 279 us with 60 dims rotated, 81 with 64).
 //
 // Measured (B200, graph replay): 16383 tokens of 48 heads x 128, bf16, 64 dims rotated interleaved, 81 us (5.0 TB/s); of 48 x 64, fp32 to
 // fp16, in halves, 69 us (5.4 TB/s); 64 tokens of one step 2.9 us.

@@ -14,7 +14,8 @@ over beams, per step:
 Every call enqueues its work on the current stream of the cache's device, reads lengths, tables and parents there
 (nothing is copied to the host or waited for) and returns new tensors unless `out` is given. Errors in what the
 host can see raise CudaLLMError (INVALID_ARG) before anything runs; contents out of range are bounded as
-include/cudallm.h states. A cache serves one host thread at a time.
+include/cudallm.h states. A cache serves one host thread at a time. No gradient flows through these calls: outputs are detached from
+inputs that require one.
 """
 from __future__ import annotations
 
@@ -172,8 +173,9 @@ class Rope:
              low: float = 1.0, high: float | None = None, interleaved: bool = False, device="cuda") -> "Rope":
         """Frequencies theta^(-2j / rotary), for contexts `scale` times the `original` length: "linear" divides all of them by
         `scale`; "llama3" and "yarn" divide those that turn fewer than `low` times within `original` positions, keep
-        those that turn more than `high` times (4 and 32) and blend between; yarn also multiplies cos and sin by
-        0.1 ln(scale) + 1."""
+        those that turn more than `high` times (4 and 32) and blend between, linearly in the number of turns; yarn also
+        multiplies cos and sin by 0.1 ln(scale) + 1. Some loaders of yarn checkpoints blend linearly in the index of the
+        pair between the same two ends instead, which gives other frequencies: pass theirs to Rope itself."""
         _need(rotary > 0 and rotary % 2 == 0, "rotary must be positive and even")
         _need(scaling in ("none", "linear", "llama3", "yarn"), "scaling must be none, linear, llama3 or yarn")
         f = theta ** (-torch.arange(0, rotary, 2, dtype=torch.float64) / rotary)
